@@ -112,6 +112,12 @@ class PagedKvAddress(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in ("physical_page", "offset_in_page", "generation")]
 
 
+class PagedBatchRaw(C.Structure):
+    """flat_paged_batch: a batch of sequences whose lengths and page tables stay on the device."""
+    _fields_ = [(n, C.c_uint64) for n in ("num_seqs", "page_size", "physical_pages", "max_pages_per_seq")] + \
+               [(n, C.c_void_p) for n in ("page_tables", "page_counts", "context_lens", "free_pages", "free_count")]
+
+
 class BackwardLayout(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in ("q_elements", "kv_elements", "lse_elements", "q_offset", "k_offset",
                                             "v_offset", "d_out_offset", "out_offset", "lse_offset", "input_bytes",
@@ -147,6 +153,13 @@ def lib() -> C.CDLL:
                      "flat_prepared_backward_destroy", "flat_splitkv_exchange_destroy"):
             getattr(_lib, name).restype = None
             getattr(_lib, name).argtypes = [C.c_void_p]
+        # the calls of a serving step on device-resident batches are short: no conversion by hand
+        ptr, u64, i32 = C.c_void_p, C.c_uint64, C.c_int32
+        _lib.flat_paged_batch_reserve.argtypes = [ptr, ptr, ptr, ptr, u64] + [ptr] * 6
+        _lib.flat_paged_batch_release.argtypes = [ptr] * 5
+        _lib.flat_paged_kv_write.argtypes = [ptr, i32, u64, u64, u64, u64, ptr, ptr, C.c_float] + [Buffer] * 4
+        _lib.flat_paged_kv_accept.argtypes = [ptr, i32, ptr, u64, u64, u64, ptr, ptr, ptr, Buffer, Buffer]
+        _lib.flat_decode_paged_tree.argtypes = [ptr, i32, ptr] + [u64] * 6 + [ptr, ptr, ptr, u64, ptr, C.c_float] + [Buffer] * 4
     return _lib
 
 
@@ -461,6 +474,64 @@ class Context:
         self.check(lib().flat_splitkv_merge(self.h, C.c_int32(dtype), C.c_uint64(parts), C.c_uint64(rows),
                                             C.c_uint64(head_dim), buf(partial_o), buf(partial_lse), buf(out)))
 
+    # ---- batches whose lengths and page tables stay on the device ----
+    def paged_batch_reserve(self, batch: "PagedBatch", new_lens, max_new_tokens: int, new_offsets, slot_map, positions, depths=None,
+                            page_counts_out=None, free_count_out=None, context_lens_out=None):
+        """Pages and slots for new_lens[s] tokens behind each sequence's live ones (flat_paged_batch_reserve); outputs None: in place,
+        context_lens_out None: not written."""
+        _ints(batch.num_seqs, new_lens=new_lens, page_counts_out=page_counts_out, context_lens_out=context_lens_out)
+        _ints(max_new_tokens, slot_map=slot_map, positions=positions, depths=depths)
+        _ints(batch.num_seqs + 1, new_offsets=new_offsets)
+        _ints(1, free_count_out=free_count_out)
+        self.check(lib().flat_paged_batch_reserve(self.h, batch.ref, _p(new_lens), _p(depths), max_new_tokens, _p(page_counts_out),
+                                                  _p(free_count_out), _p(context_lens_out), _p(new_offsets), _p(slot_map), _p(positions)))
+
+    def paged_batch_release(self, batch: "PagedBatch", keep_lens, page_counts_out=None, free_count_out=None):
+        """Gives back each sequence's pages behind its first keep_lens[s] tokens (flat_paged_batch_release)."""
+        _ints(batch.num_seqs, keep_lens=keep_lens, page_counts_out=page_counts_out)
+        _ints(1, free_count_out=free_count_out)
+        self.check(lib().flat_paged_batch_release(self.h, batch.ref, _p(keep_lens), _p(page_counts_out), _p(free_count_out)))
+
+    def paged_kv_write(self, kv_heads: int, head_dim: int, slot_map, positions, theta: float, k_source, v_source, k, v):
+        """New tokens' K (turned at `positions`; None: as it is) and V into the pool rows that slot_map names (flat_paged_kv_write).
+        k_source / v_source [tokens, kv_heads*head_dim], k / v [pool_rows, kv_heads*head_dim]."""
+        tokens = slot_map.numel()
+        _ints(tokens, slot_map=slot_map, positions=positions)
+        _same_type(k_source, v_source, k, v)
+        pool_rows = _b(k).bytes // (kv_heads * head_dim * k_source.element_size()) if kv_heads * head_dim else 0
+        self.check(lib().flat_paged_kv_write(self.h, _dtype_of(k_source), tokens, kv_heads, head_dim, pool_rows, _p(slot_map), _p(positions),
+                                             theta, _whole(k_source), _whole(v_source), _whole(k), _whole(v)))
+
+    def decode_paged_tree(self, batch: "PagedBatch", q_heads: int, kv_heads: int, head_dim: int, max_nodes: int, max_context: int, q_offsets,
+                          q_positions, tree_mask, cfg, theta: float, q, k, v, out):
+        """Attention of drafted tokens, packed sequence by sequence in `q` [tokens, q_heads*head_dim], over the cache that holds
+        them behind each sequence's live tokens (flat_decode_paged_tree).  tree_mask: int32 [tokens, words] of bits, or None.  `out`:
+        create_decode_output_buffer(dtype, tokens, q_heads, head_dim)."""
+        tokens = q_positions.numel()
+        _ints(batch.num_seqs + 1, q_offsets=q_offsets)
+        _ints(tokens, q_positions=q_positions)
+        words = 0
+        if tree_mask is not None:
+            if tree_mask.dim() != 2 or tree_mask.shape[0] != tokens:
+                raise FlatAttentionError(7, f"tree_mask has shape {tuple(tree_mask.shape)}, expected [{tokens}, words]")
+            words = tree_mask.shape[1]
+            _ints(tokens * words, tree_mask=tree_mask)
+        _same_type(q, k, v)
+        self.check(lib().flat_decode_paged_tree(self.h, _dtype_of(q), batch.ref, q_heads, kv_heads, head_dim, tokens, max_nodes, max_context,
+                                                _p(q_offsets), _p(q_positions), _p(tree_mask), words, C.byref(cfg), theta, _whole(q), _whole(k),
+                                                _whole(v), _whole(out)))
+
+    def paged_kv_accept(self, batch: "PagedBatch", kv_heads: int, head_dim: int, accept_nodes, accept_lens, context_lens_out, k, v):
+        """Moves the rows of each sequence's accepted path (accept_nodes [num_seqs, max_accept], the first accept_lens[s] of a row) behind
+        its live tokens and lengthens it (flat_paged_kv_accept); context_lens_out None: in place."""
+        if accept_nodes.dim() != 2 or accept_nodes.shape[0] != batch.num_seqs:
+            raise FlatAttentionError(7, f"accept_nodes has shape {tuple(accept_nodes.shape)}, expected [{batch.num_seqs}, max_accept]")
+        _ints(accept_nodes.numel(), accept_nodes=accept_nodes)
+        _ints(batch.num_seqs, accept_lens=accept_lens, context_lens_out=context_lens_out)
+        dtype = _same_type(k, v)
+        self.check(lib().flat_paged_kv_accept(self.h, batch.dtype if dtype is None else dtype, batch.ref, kv_heads, head_dim,
+                                              accept_nodes.shape[1], _p(accept_nodes), _p(accept_lens), _p(context_lens_out), _whole(k), _whole(v)))
+
     def chunked_prefill(self, dtype, shp, cfg, rot, query_chunk_size, q, k, v, out):
         self.check(lib().flat_chunked_prefill(self.h, C.c_int32(dtype), C.byref(shp), C.byref(cfg), C.byref(rot),
                                               C.c_uint64(query_chunk_size), buf(q), buf(k), buf(v), buf(out)))
@@ -560,6 +631,69 @@ class PreparedBackward:
 
 def _b(x) -> Buffer:
     return x if isinstance(x, Buffer) else buf(x)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _ints(elements: int, **tensors):
+    """Each given tensor is a contiguous int32 CUDA tensor of at least `elements`."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.dtype != _torch().int32:
+            raise FlatAttentionError(26, f"{name} must be int32, is {t.dtype}")
+        if not t.is_cuda or not t.is_contiguous():
+            raise FlatAttentionError(29, f"{name} must be a contiguous CUDA tensor")
+        if t.numel() < elements:
+            raise FlatAttentionError(22, f"{name} has {t.numel()} elements, requires {elements}")
+
+
+def _same_type(*tensors):
+    """Tensors (flat_buffer views have no type) share one; returns its dtype code, None if all are views."""
+    code = None
+    for t in tensors:
+        if isinstance(t, Buffer):
+            continue
+        c = _dtype_of(t)
+        if code is not None and c != code:
+            raise FlatAttentionError(26, "Q, K and V differ in type")
+        code = c
+    return code
+
+
+def _whole(x) -> Buffer:
+    """A contiguous CUDA tensor or a flat_buffer view."""
+    if isinstance(x, Buffer):
+        return x
+    if not x.is_cuda or not x.is_contiguous():
+        raise FlatAttentionError(29, "tensors must be contiguous and on the device")
+    return buf(x)
+
+
+class PagedBatch:
+    """A batch of sequences over one pool of pages, its page tables, lengths and free pages in device memory (flat_paged_batch).
+    Tensors that are not given start empty: no sequence holds a page, and all pages of the pool are free, the lowest on top."""
+
+    def __init__(self, num_seqs: int, page_size: int, physical_pages: int, max_pages_per_seq: int, page_tables=None, page_counts=None,
+                 context_lens=None, free_pages=None, free_count=None, device: int = 0, dtype: int = BF16):
+        torch = _torch()
+        on = dict(dtype=torch.int32, device=f"cuda:{device}")
+        self.num_seqs, self.page_size, self.physical_pages, self.max_pages_per_seq = num_seqs, page_size, physical_pages, max_pages_per_seq
+        self.dtype = dtype  # of the pool, where calls are given flat_buffer views instead of tensors
+        self.page_tables = torch.full((num_seqs, max_pages_per_seq), -1, **on) if page_tables is None else page_tables
+        self.page_counts = torch.zeros(num_seqs, **on) if page_counts is None else page_counts
+        self.context_lens = torch.zeros(num_seqs, **on) if context_lens is None else context_lens
+        self.free_pages = torch.arange(physical_pages - 1, -1, -1, **on) if free_pages is None else free_pages
+        self.free_count = torch.full((1,), physical_pages, **on) if free_count is None else free_count
+        _ints(num_seqs * max_pages_per_seq, page_tables=self.page_tables)
+        _ints(num_seqs, page_counts=self.page_counts, context_lens=self.context_lens)
+        _ints(physical_pages, free_pages=self.free_pages)
+        _ints(1, free_count=self.free_count)
+        self.raw = PagedBatchRaw(num_seqs, page_size, physical_pages, max_pages_per_seq, *(
+            t.data_ptr() for t in (self.page_tables, self.page_counts, self.context_lens, self.free_pages, self.free_count)))
+        self.ref = C.byref(self.raw)
 
 
 # ---- PagedKvTable (src/paged_kv.rs:75-188) -----------------------------------------------------

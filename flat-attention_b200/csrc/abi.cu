@@ -7,6 +7,7 @@
 #include <new>
 
 #include "common.h"
+#include "turns.cuh"
 
 namespace flat {
 
@@ -42,6 +43,20 @@ int ensure_host_stage(flat_ctx *ctx, uint64_t need) {
     FLAT_CUDA_OK(ctx, cudaMalloc(&ctx->host_stage, need));
     ctx->host_stage_bytes = need;
     return FLAT_OK;
+}
+
+// The scratch of the calls on device-resident batches.  Not while the stream is captured: an allocation would end the capture.
+int ensure_paged_scratch(flat_ctx *ctx) {
+    if (ctx->paged_scratch) return FLAT_OK;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    FLAT_CUDA_OK(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
+    if (capture != cudaStreamCaptureStatusNone)
+        return fail(ctx, FLAT_ERR_EXECUTION, "the first call on a device-resident batch allocates its scratch: make one before the capture");
+    cudaError_t e = cudaMalloc(&ctx->paged_scratch, kPagedScratchBytes);
+    if (e == cudaSuccess) return FLAT_OK;
+    cudaGetLastError();
+    ctx->paged_scratch = nullptr;
+    return fail(ctx, FLAT_ERR_EXECUTION, "cudaMalloc of %llu bytes failed: %s", (unsigned long long)kPagedScratchBytes, cudaGetErrorString(e));
 }
 
 namespace {
@@ -644,6 +659,7 @@ void flat_ctx_destroy(flat_ctx *ctx) {
         if (t.dev) cudaFree(t.dev);
     if (ctx->f32_table.dev) cudaFree(ctx->f32_table.dev);
     if (ctx->short_partials) cudaFree(ctx->short_partials);
+    if (ctx->paged_scratch) cudaFree(ctx->paged_scratch);
     for (cudaEvent_t e : ctx->pipe_events) cudaEventDestroy(e);
     if (ctx->stream_switch) cudaEventDestroy(ctx->stream_switch);
     if (ctx->copy_in) cudaStreamDestroy(ctx->copy_in);
@@ -756,6 +772,12 @@ int32_t flat_ctx_device_status(flat_ctx *ctx) {
             fail(ctx, h.code, "a page-table entry of sequence %d lies outside the physical pool; its tokens were masked", h.where);
         else if (h.code == FLAT_ERR_NON_FINITE_INPUT)
             fail(ctx, h.code, "a device-side input scan found a non-finite value (tensor %d)", h.where);
+        else if (h.code == FLAT_ERR_CAPACITY_EXCEEDED)
+            fail(ctx, h.code, "the free pages do not hold the new tokens of sequence %d", h.where);
+        else if (h.code == FLAT_ERR_CAPACITY_OVERFLOW)
+            fail(ctx, h.code, "the count of free pages leaves the pool (sequence %d)", h.where);
+        else if (h.code == FLAT_ERR_INVALID_CACHE_LENGTH || h.code == FLAT_ERR_LENGTH_MISMATCH)
+            fail(ctx, h.code, "lengths of sequence %d do not fit its pages or the call's bounds; it was left out", h.where);
         else
             fail(ctx, h.code, "device wait expired at site %d", h.where);
         cudaMemset(ctx->dev_status, 0, sizeof(DeviceStatus));
@@ -1749,6 +1771,269 @@ int32_t flat_splitkv_merge(flat_ctx *ctx, int32_t dtype, uint64_t parts, uint64_
                                 static_cast<const float *>(partial_o.ptr), static_cast<const float *>(partial_lse.ptr),
                                 (int64_t)(rows * head_dim), (int64_t)rows, out_and_lse.ptr,
                                 reinterpret_cast<float *>(static_cast<char *>(out_and_lse.ptr) + lse_off));
+}
+
+// ---- batches whose lengths and page tables stay on the device ----------------------------------
+}  // extern "C"
+
+namespace {
+
+// Launches go to the context's device whatever device is current.
+struct DeviceGuard {
+    int before = -1;
+    explicit DeviceGuard(const flat_ctx *ctx) {
+        int current = -1;
+        if (cudaGetDevice(&current) == cudaSuccess && current != ctx->device && cudaSetDevice(ctx->device) == cudaSuccess) before = current;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+int check_ints(flat_ctx *ctx, const char *name, const int32_t *p) {
+    if (!p) return fail(ctx, FLAT_ERR_NULL_POINTER, "%s is null", name);
+    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(ctx, FLAT_ERR_MISALIGNED_BUFFER, "%s must be 4-byte aligned", name);
+    return FLAT_OK;
+}
+int check_optional_ints(flat_ctx *ctx, const char *name, const int32_t *p) { return p ? check_ints(ctx, name, p) : FLAT_OK; }
+
+int check_elements(flat_ctx *ctx, const char *name, flat_buffer b, uint64_t required, uint64_t size) {
+    if (int st = check_buffer(ctx, name, b, required)) return st;
+    if (reinterpret_cast<uintptr_t>(b.ptr) % size) return fail(ctx, FLAT_ERR_MISALIGNED_BUFFER, "%s buffer must be aligned to its elements", name);
+    return FLAT_OK;
+}
+
+int validate_batch(flat_ctx *ctx, const flat_paged_batch *b) {
+    if (!b) return fail(ctx, FLAT_ERR_NULL_POINTER, "batch is null");
+    if (b->num_seqs == 0 || b->page_size == 0 || b->physical_pages == 0 || b->max_pages_per_seq == 0)
+        return fail(ctx, FLAT_ERR_ZERO_DIMENSION, "paged batch dimensions must all be non-zero");
+    const uint64_t lim = (uint64_t)std::numeric_limits<int32_t>::max();
+    uint64_t rows;
+    if (b->num_seqs > kMaxBatchSeqs) return fail(ctx, FLAT_ERR_DISPATCH_LIMIT, "batch of %llu sequences exceeds %llu", (unsigned long long)b->num_seqs,
+                                                 (unsigned long long)kMaxBatchSeqs);
+    if (b->max_pages_per_seq > lim || !mul_ok(b->page_size, b->physical_pages, &rows) || rows > lim)
+        return fail(ctx, FLAT_ERR_INDEX_SPACE_EXCEEDED, "paged batch geometry exceeds the index space");
+    return FLAT_OK;
+}
+
+// head_dim and heads of the rows of a pool; *row receives kv_heads * head_dim
+int validate_rows(flat_ctx *ctx, int dtype, uint64_t pool_rows, uint64_t kv_heads, uint64_t head_dim, flat_buffer k, flat_buffer v, uint64_t *row) {
+    if (int st = check_dtype(ctx, dtype)) return st;
+    if (kv_heads == 0 || head_dim == 0) return fail(ctx, FLAT_ERR_ZERO_DIMENSION, "pool dimensions must be non-zero");
+    uint64_t bytes;
+    const uint64_t size = dtype_size(dtype);
+    if (kv_heads > (uint64_t)1 << 20 || head_dim > (uint64_t)1 << 10)
+        return fail(ctx, FLAT_ERR_INDEX_SPACE_EXCEEDED, "%llu heads of %llu values exceed the index space", (unsigned long long)kv_heads, (unsigned long long)head_dim);
+    *row = kv_heads * head_dim;
+    if (!mul_ok(pool_rows, *row * size, &bytes)) return fail(ctx, FLAT_ERR_SHAPE_OVERFLOW, "pool size overflows");
+    if (int st = check_elements(ctx, "K", k, bytes, size)) return st;
+    return check_elements(ctx, "V", v, bytes, size);
+}
+
+PagedBatchParams batch_params(flat_ctx *ctx, const flat_paged_batch *b) {
+    PagedBatchParams p{};
+    p.num_seqs = (int)b->num_seqs;
+    p.page_size = (int)b->page_size;
+    p.physical_pages = (int)b->physical_pages;
+    p.max_pages = (int)b->max_pages_per_seq;
+    p.page_tables = b->page_tables;
+    p.page_counts = b->page_counts;
+    p.context_lens = b->context_lens;
+    p.free_pages = b->free_pages;
+    p.free_count = b->free_count;
+    p.status = ctx->dev_status;
+    p.plan = static_cast<int4 *>(ctx->paged_scratch);
+    p.plan_offsets = reinterpret_cast<int32_t *>(p.plan + kMaxBatchSeqs + 1);
+    p.plan_free_count = p.plan_offsets + kMaxBatchSeqs + 1;
+    static_assert((kMaxBatchSeqs + 1) * (sizeof(int4) + sizeof(int32_t)) + sizeof(int32_t) <= kPagedPlanBytes, "plan region");
+    return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t flat_paged_batch_reserve(flat_ctx *ctx, const flat_paged_batch *batch, const int32_t *new_lens_dev, const int32_t *depths_dev,
+                                 uint64_t max_new_tokens, int32_t *page_counts_out, int32_t *free_count_out, int32_t *context_lens_out,
+                                 int32_t *new_offsets_dev, int32_t *slot_map_dev, int32_t *positions_dev) {
+    if (!ctx) return FLAT_ERR_NULL_POINTER;
+    int st;
+    if ((st = validate_batch(ctx, batch))) return st;
+    if (max_new_tokens == 0) return fail(ctx, FLAT_ERR_ZERO_DIMENSION, "max_new_tokens must be non-zero");
+    if (max_new_tokens > (uint64_t)std::numeric_limits<int32_t>::max())
+        return fail(ctx, FLAT_ERR_INDEX_SPACE_EXCEEDED, "max_new_tokens %llu exceeds the index space", (unsigned long long)max_new_tokens);
+    if ((st = check_ints(ctx, "page_tables", batch->page_tables)) || (st = check_ints(ctx, "page_counts", batch->page_counts)) ||
+        (st = check_ints(ctx, "context_lens", batch->context_lens)) || (st = check_ints(ctx, "free_pages", batch->free_pages)) ||
+        (st = check_ints(ctx, "free_count", batch->free_count)) || (st = check_ints(ctx, "new_lens", new_lens_dev)) ||
+        (st = check_optional_ints(ctx, "depths", depths_dev)) || (st = check_optional_ints(ctx, "page_counts_out", page_counts_out)) ||
+        (st = check_optional_ints(ctx, "free_count_out", free_count_out)) || (st = check_optional_ints(ctx, "context_lens_out", context_lens_out)) ||
+        (st = check_ints(ctx, "new_offsets", new_offsets_dev)) || (st = check_ints(ctx, "slot_map", slot_map_dev)) ||
+        (st = check_ints(ctx, "positions", positions_dev)))
+        return st;
+    const DeviceGuard guard(ctx);
+    if ((st = ensure_paged_scratch(ctx))) return st;
+    PagedBatchParams p = batch_params(ctx, batch);
+    p.lens = new_lens_dev;
+    p.depths = depths_dev;
+    p.max_tokens = (int)max_new_tokens;
+    p.page_counts_out = page_counts_out ? page_counts_out : batch->page_counts;
+    p.free_count_out = free_count_out ? free_count_out : batch->free_count;
+    p.context_lens_out = context_lens_out;
+    p.offsets = new_offsets_dev;
+    p.slots = slot_map_dev;
+    p.positions = positions_dev;
+    return launch_paged_batch(ctx, p, false);
+}
+
+int32_t flat_paged_batch_release(flat_ctx *ctx, const flat_paged_batch *batch, const int32_t *keep_lens_dev, int32_t *page_counts_out,
+                                 int32_t *free_count_out) {
+    if (!ctx) return FLAT_ERR_NULL_POINTER;
+    int st;
+    if ((st = validate_batch(ctx, batch))) return st;
+    if ((st = check_ints(ctx, "page_tables", batch->page_tables)) || (st = check_ints(ctx, "page_counts", batch->page_counts)) ||
+        (st = check_ints(ctx, "free_pages", batch->free_pages)) || (st = check_ints(ctx, "free_count", batch->free_count)) ||
+        (st = check_ints(ctx, "keep_lens", keep_lens_dev)) || (st = check_optional_ints(ctx, "page_counts_out", page_counts_out)) ||
+        (st = check_optional_ints(ctx, "free_count_out", free_count_out)))
+        return st;
+    const DeviceGuard guard(ctx);
+    if ((st = ensure_paged_scratch(ctx))) return st;
+    PagedBatchParams p = batch_params(ctx, batch);
+    p.lens = keep_lens_dev;
+    p.page_counts_out = page_counts_out ? page_counts_out : batch->page_counts;
+    p.free_count_out = free_count_out ? free_count_out : batch->free_count;
+    return launch_paged_batch(ctx, p, true);
+}
+
+int32_t flat_paged_kv_write(flat_ctx *ctx, int32_t dtype, uint64_t tokens, uint64_t kv_heads, uint64_t head_dim, uint64_t pool_rows,
+                            const int32_t *slot_map_dev, const int32_t *positions_dev, float theta, flat_buffer k_source,
+                            flat_buffer v_source, flat_buffer k, flat_buffer v) {
+    if (!ctx) return FLAT_ERR_NULL_POINTER;
+    int st;
+    uint64_t row;
+    const uint64_t lim = (uint64_t)std::numeric_limits<int32_t>::max();
+    if (tokens == 0 || pool_rows == 0) return fail(ctx, FLAT_ERR_ZERO_DIMENSION, "tokens and pool_rows must be non-zero");
+    if (tokens > lim || pool_rows > lim) return fail(ctx, FLAT_ERR_INDEX_SPACE_EXCEEDED, "tokens or pool_rows exceed the index space");
+    if ((st = validate_rows(ctx, dtype, pool_rows, kv_heads, head_dim, k, v, &row))) return st;
+    const uint64_t size = dtype_size(dtype);
+    if ((st = check_elements(ctx, "K source", k_source, tokens * row * size, size)) ||
+        (st = check_elements(ctx, "V source", v_source, tokens * row * size, size)) || (st = check_ints(ctx, "slot_map", slot_map_dev)) ||
+        (st = check_optional_ints(ctx, "positions", positions_dev)))
+        return st;
+    PagedWriteParams p{};
+    if (positions_dev) {
+        if (head_dim > (uint64_t)kMaxHeadDim)
+            return fail(ctx, FLAT_ERR_UNSUPPORTED_HEAD_DIM, "head_dim %llu exceeds maximum %d", (unsigned long long)head_dim, kMaxHeadDim);
+        if ((st = validate_rotary(ctx, theta, 0, head_dim, 1))) return st;
+        fill_turns(ctx, theta, (int)head_dim, &p.freq);
+    }
+    const DeviceGuard guard(ctx);
+    p.k_src = k_source.ptr;
+    p.v_src = v_source.ptr;
+    p.k_dst = k.ptr;
+    p.v_dst = v.ptr;
+    p.slots = slot_map_dev;
+    p.positions = positions_dev;
+    p.tokens = (int64_t)tokens;
+    p.pool_rows = (int64_t)pool_rows;
+    p.row_elems = (int)row;
+    p.head_dim = (int)head_dim;
+    p.status = ctx->dev_status;
+    return launch_paged_write(ctx, dtype, p);
+}
+
+int32_t flat_paged_kv_accept(flat_ctx *ctx, int32_t dtype, const flat_paged_batch *batch, uint64_t kv_heads, uint64_t head_dim,
+                             uint64_t max_accept, const int32_t *accept_nodes_dev, const int32_t *accept_lens_dev,
+                             int32_t *context_lens_out, flat_buffer k, flat_buffer v) {
+    if (!ctx) return FLAT_ERR_NULL_POINTER;
+    int st;
+    uint64_t row;
+    if ((st = validate_batch(ctx, batch))) return st;
+    if (max_accept == 0) return fail(ctx, FLAT_ERR_ZERO_DIMENSION, "max_accept must be non-zero");
+    if (max_accept > (uint64_t)std::numeric_limits<int32_t>::max())
+        return fail(ctx, FLAT_ERR_INDEX_SPACE_EXCEEDED, "max_accept %llu exceeds the index space", (unsigned long long)max_accept);
+    if ((st = validate_rows(ctx, dtype, batch->page_size * batch->physical_pages, kv_heads, head_dim, k, v, &row))) return st;
+    if ((st = check_ints(ctx, "page_tables", batch->page_tables)) || (st = check_ints(ctx, "page_counts", batch->page_counts)) ||
+        (st = check_ints(ctx, "context_lens", batch->context_lens)) || (st = check_ints(ctx, "accept_nodes", accept_nodes_dev)) ||
+        (st = check_ints(ctx, "accept_lens", accept_lens_dev)) || (st = check_optional_ints(ctx, "context_lens_out", context_lens_out)))
+        return st;
+    const DeviceGuard guard(ctx);
+    PagedAcceptParams p{};
+    p.k = k.ptr;
+    p.v = v.ptr;
+    p.num_seqs = (int)batch->num_seqs;
+    p.page_size = (int)batch->page_size;
+    p.physical_pages = (int)batch->physical_pages;
+    p.max_pages = (int)batch->max_pages_per_seq;
+    p.max_accept = (int)max_accept;
+    p.page_tables = batch->page_tables;
+    p.page_counts = batch->page_counts;
+    p.context_lens = batch->context_lens;
+    p.path = accept_nodes_dev;
+    p.accept_lens = accept_lens_dev;
+    p.context_lens_out = context_lens_out ? context_lens_out : batch->context_lens;
+    p.status = ctx->dev_status;
+    return launch_paged_accept(ctx, dtype, (int64_t)row, p);
+}
+
+int32_t flat_decode_paged_tree(flat_ctx *ctx, int32_t dtype, const flat_paged_batch *batch, uint64_t q_heads, uint64_t kv_heads,
+                               uint64_t head_dim, uint64_t max_q_tokens, uint64_t max_nodes, uint64_t max_context,
+                               const int32_t *q_offsets_dev, const int32_t *q_positions_dev, const int32_t *tree_mask_dev,
+                               uint64_t mask_words, const flat_attention_config *config, float theta, flat_buffer q, flat_buffer k,
+                               flat_buffer v, flat_buffer out_and_lse) {
+    if (!ctx) return FLAT_ERR_NULL_POINTER;
+    int st;
+    uint64_t row;
+    float scale;
+    if ((st = validate_batch(ctx, batch))) return st;
+    if ((st = validate_decode_geometry(ctx, q_heads, kv_heads, head_dim, theta))) return st;
+    if (max_q_tokens == 0 || max_nodes == 0 || max_context == 0)
+        return fail(ctx, FLAT_ERR_ZERO_DIMENSION, "max_q_tokens, max_nodes and max_context must be non-zero");
+    if (max_nodes > 65535 || max_q_tokens > (uint64_t)1 << 26 || max_context > (uint64_t)1 << 30)
+        return fail(ctx, FLAT_ERR_INDEX_SPACE_EXCEEDED, "drafted tokens or context exceed the index space");
+    if (tree_mask_dev && (max_nodes > 32 * std::min<uint64_t>(mask_words, 2048) || mask_words > 2048))
+        return fail(ctx, FLAT_ERR_LENGTH_MISMATCH, "tree_mask rows of %llu words do not hold %llu drafted tokens", (unsigned long long)mask_words,
+                    (unsigned long long)max_nodes);
+    if ((st = resolve_scale(ctx, config, head_dim, &scale))) return st;
+    if ((st = validate_rows(ctx, dtype, batch->page_size * batch->physical_pages, kv_heads, head_dim, k, v, &row))) return st;
+    flat_decode_layout layout;
+    if ((st = flat_decode_layout_for(dtype, max_q_tokens, q_heads, head_dim, &layout))) return fail(ctx, st, "attention shape overflows the address space");
+    const uint64_t size = dtype_size(dtype);
+    if ((st = check_elements(ctx, "Q", q, layout.q_bytes, size)) || (st = check_elements(ctx, "O|LSE", out_and_lse, layout.combined_bytes, 4)) ||
+        (st = check_ints(ctx, "page_tables", batch->page_tables)) || (st = check_ints(ctx, "page_counts", batch->page_counts)) ||
+        (st = check_ints(ctx, "context_lens", batch->context_lens)) || (st = check_ints(ctx, "q_offsets", q_offsets_dev)) ||
+        (st = check_ints(ctx, "q_positions", q_positions_dev)) || (st = check_optional_ints(ctx, "tree_mask", tree_mask_dev)))
+        return st;
+    const DeviceGuard guard(ctx);
+    if ((st = ensure_paged_scratch(ctx))) return st;
+    TreeParams p{};
+    p.q = q.ptr;
+    p.k = k.ptr;
+    p.v = v.ptr;
+    p.o = out_and_lse.ptr;
+    p.lse = reinterpret_cast<float *>(static_cast<char *>(out_and_lse.ptr) + layout.lse_byte_offset);
+    p.num_seqs = (int)batch->num_seqs;
+    p.q_heads = (int)q_heads;
+    p.kv_heads = (int)kv_heads;
+    p.head_dim = (int)head_dim;
+    p.group = (int)(q_heads / kv_heads);
+    p.page_size = (int)batch->page_size;
+    p.physical_pages = (int)batch->physical_pages;
+    p.max_pages = (int)batch->max_pages_per_seq;
+    p.max_q = (int)max_q_tokens;
+    p.max_nodes = (int)max_nodes;
+    p.max_context = (int)max_context;
+    p.page_tables = batch->page_tables;
+    p.page_counts = batch->page_counts;
+    p.context_lens = batch->context_lens;
+    p.q_offsets = q_offsets_dev;
+    p.positions = q_positions_dev;
+    p.mask = reinterpret_cast<const uint32_t *>(tree_mask_dev);
+    p.mask_words = (int)mask_words;
+    p.causal = config->causal ? 1 : 0;
+    p.scale = scale;
+    p.status = ctx->dev_status;
+    fill_turns(ctx, theta, p.head_dim, &p.freq);
+    return launch_tree_simt(ctx, dtype, p);
 }
 
 // ---- chunked prefill -------------------------------------------------------------------------

@@ -69,6 +69,10 @@ struct flat_ctx {
     // The tensor-core backward may keep every bf16 dS^T tile in scratch (O(N^2) bytes) so that dQ needs no second score
     // recompute; it does so while that spill fits this budget (flat_ctx_set_backward_scratch_budget).
     uint64_t backward_scratch_budget = 8ull << 30;
+    uint64_t turns[64] = {};  // the last table of RoPE frequencies made on the host (turns.cuh): 64 powers cost 10 us of a call
+    float turns_theta = 0.f;
+    int turns_dim = 0;
+    void *paged_scratch = nullptr;  // of the calls on device-resident batches, kPagedScratchBytes once one has been made
     cudaEvent_t stream_switch = nullptr;  // orders the old and the new stream in flat_ctx_set_stream
     // sequence offsets of the last balanced decode plan and where they were uploaded (skips identical re-uploads)
     std::vector<int32_t> plan_offsets;
@@ -302,6 +306,73 @@ int launch_append_rows(flat_ctx *ctx, int dtype, const void *k_src, const void *
                        void *v_dst, void *k_shadow, int64_t rows, int row_elems, int head_dim,
                        const int32_t *page_table, int page_size, int64_t first_logical,
                        int64_t dst_row0, int rotate, int64_t pos0, const float *inv_freq);
+
+// ---- batches on the device -------------------------------------------------------------------
+// Scratch of these calls: a block of its own of fixed size, allocated by the first call and never moved, so that captured launches
+// stay valid whatever is called later.
+constexpr uint64_t kPagedScratchBytes = 48ull << 20;
+constexpr uint64_t kPagedPlanBytes = 2ull << 20;  // plans of reserve and release, at its start: 20 bytes a sequence
+constexpr uint64_t kMaxBatchSeqs = 65535;
+int ensure_paged_scratch(flat_ctx *ctx);
+struct PagedBatchParams {
+    int num_seqs, page_size, physical_pages, max_pages;
+    int32_t *page_tables;
+    const int32_t *page_counts, *context_lens;
+    int32_t *free_pages;
+    const int32_t *free_count;
+    const int32_t *lens;    // reserve: new tokens, release: tokens to keep
+    const int32_t *depths;  // reserve, optional: position of each new token behind the live ones
+    int max_tokens;         // reserve: entries of slots and positions
+    int32_t *page_counts_out, *free_count_out, *context_lens_out;
+    int32_t *offsets, *slots, *positions;
+    int4 *plan;             // scratch, per sequence.  reserve: live tokens, held pages, pages given before, granted; release: -, held pages, pages left, -
+    int32_t *plan_offsets;  // scratch, release: where each sequence's pages go, [num_seqs + 1]
+    int32_t *plan_free_count;
+    DeviceStatus *status;
+    int fused;
+};
+int launch_paged_batch(flat_ctx *ctx, PagedBatchParams &p, bool release);
+struct TurnTable {
+    uint64_t turns[kMaxHeadDim / 2];  // see turns.cuh
+};
+struct PagedWriteParams {
+    const void *k_src, *v_src;
+    void *k_dst, *v_dst;
+    const int32_t *slots, *positions;  // positions null: K is stored as it is
+    int64_t tokens, pool_rows;
+    int row_elems, head_dim;
+    int block_tokens;
+    TurnTable freq;
+    DeviceStatus *status;
+};
+int launch_paged_write(flat_ctx *ctx, int dtype, PagedWriteParams &p);
+struct PagedAcceptParams {
+    void *k, *v;
+    int num_seqs, page_size, physical_pages, max_pages, max_accept;
+    const int32_t *page_tables, *page_counts, *context_lens, *path, *accept_lens;
+    int32_t *context_lens_out;
+    int64_t row_vecs;
+    DeviceStatus *status;
+};
+int launch_paged_accept(flat_ctx *ctx, int dtype, int64_t row_elems, PagedAcceptParams &p);
+struct TreeParams {
+    const void *q, *k, *v;
+    void *o;
+    float *lse;
+    int num_seqs, q_heads, kv_heads, head_dim, group;
+    int page_size, physical_pages, max_pages;
+    int max_q;                          // rows of q and o
+    int max_nodes, max_context;         // of one sequence; max_context counts its drafted tokens too
+    const int32_t *page_tables, *page_counts, *context_lens, *q_offsets, *positions;
+    const uint32_t *mask;               // [max_q, mask_words]; null: `causal` says what a drafted token sees
+    int mask_words, causal;
+    float scale;
+    TurnTable freq;
+    DeviceStatus *status;
+    int splits, chunk;                  // of the generic kernel
+    float *partial_o, *partial_lse;
+};
+int launch_tree_simt(flat_ctx *ctx, int dtype, TreeParams &p);
 
 // ---- backward --------------------------------------------------------------------------------
 struct BwdParams {

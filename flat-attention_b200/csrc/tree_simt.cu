@@ -1,0 +1,293 @@
+// Attention of drafted tokens over a paged cache, any type, head_dim, group and page size, in 32-bit arithmetic.
+//
+//   query i of sequence s, turned at its position, sees the L live tokens and drafted token j (row L + j) iff its mask says so:
+//   O = softmax(scale * q K^T) V,  LSE = log sum exp;  a query that sees nothing: O = 0, LSE = -inf
+//
+// A block takes one KV head of one sequence, 32 of its (drafted token, head of the group) rows and a chunk of the tokens; it goes
+// over the chunk in tiles of 32 tokens that it holds in shared memory as f32, with the running maximum and sum of each row.  The
+// chunks' results are joined by a second kernel.  Bound by the FMA pipe for many rows and by latency for few; each K and V byte is
+// read once per 32 rows.  A masked token counts for nothing whatever its K and V hold: its score is replaced, not added to, and its
+// product with V is left out rather than formed with weight 0.
+#include "common.h"
+#include "turns.cuh"
+
+namespace flat {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kRows = 32, kTokens = 32, kThreads = 128;
+constexpr float kMasked = -1.f;  // in place of a weight, which is never negative
+
+template <typename T> __device__ __forceinline__ float to_float(T x);
+template <> __device__ __forceinline__ float to_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// What a block knows of its sequence.  The device arrays hold whatever they hold: the rows stay inside q and o, the tokens inside
+// the pages that the sequence holds.
+struct Span {
+    int first, nodes, len, tokens;  // rows of q; drafted tokens; live tokens; tokens that there are pages for
+};
+__device__ __forceinline__ Span span_of(const TreeParams &p, int seq) {
+    Span s;
+    s.first = p.q_offsets[seq];
+    s.nodes = p.q_offsets[seq + 1] - s.first;
+    s.len = p.context_lens[seq];
+    if (s.first < 0 || s.nodes <= 0 || s.nodes > p.max_nodes || s.nodes > p.max_q - s.first || s.len < 0) {
+        if (s.nodes != 0 && threadIdx.x == 0) {
+            p.status->code = FLAT_ERR_LENGTH_MISMATCH;
+            p.status->where = seq;
+        }
+        s.nodes = 0;
+        s.tokens = 0;
+        return s;
+    }
+    const int64_t room = (int64_t)min(max(p.page_counts[seq], 0), p.max_pages) * p.page_size, want = (int64_t)s.len + s.nodes;
+    s.tokens = (int)min(min(want, room), (int64_t)p.max_context);
+    if (s.tokens < want && threadIdx.x == 0) {
+        p.status->code = FLAT_ERR_PAGE_OUT_OF_RANGE;
+        p.status->where = seq;
+    }
+    return s;
+}
+
+__device__ __forceinline__ bool sees(const TreeParams &p, const Span &s, int node, int token) {
+    if (token < s.len) return true;
+    const int j = token - s.len;
+    if (j >= s.nodes) return false;
+    if (!p.mask) return !p.causal || j <= node;
+    return (p.mask[(int64_t)(s.first + node) * p.mask_words + (j >> 5)] >> (j & 31)) & 1u;
+}
+
+template <typename T> __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_constant__ TreeParams p) {
+    extern __shared__ __align__(16) float smem[];
+    grid_dependency_wait();
+    grid_dependency_launch();
+    const int tid = threadIdx.x;
+    const int D = p.head_dim, D4 = (D + 3) / 4 * 4, stride = D4 + 4;
+    float *q_s = smem, *k_s = q_s + kRows * stride, *v_s = k_s + kTokens * stride, *p_s = v_s + kTokens * stride;
+    float *m_s = p_s + kRows * (kTokens + 1), *l_s = m_s + kRows, *a_s = l_s + kRows;
+    __shared__ int64_t row_s[kTokens];
+    const int tiles = (p.max_nodes * p.group + kRows - 1) / kRows;
+    const int seq = blockIdx.z, kv_head = blockIdx.y / tiles, row0 = blockIdx.y % tiles * kRows, split = blockIdx.x;
+    const Span s = span_of(p, seq);
+    const int rows = min(kRows, s.nodes * p.group - row0);
+    if (rows <= 0) return;
+    const int begin = (int)min((int64_t)split * p.chunk, (int64_t)s.tokens), end = (int)min((int64_t)begin + p.chunk, (int64_t)s.tokens);
+    if (begin >= end && split > 0) return;  // the merge leaves it out
+
+    // the rows' queries, turned, with the softmax scale and log2(e): scores come out in the exp2 domain
+    for (int i = tid; i < kRows * (stride / 2); i += kThreads) {
+        const int r = i / (stride / 2), e = i % (stride / 2) * 2;
+        float x = 0.f, y = 0.f;
+        if (r < rows && e < D) {
+            const int node = s.first + (row0 + r) / p.group, head = kv_head * p.group + (row0 + r) % p.group;
+            const T *at = static_cast<const T *>(p.q) + ((int64_t)node * p.q_heads + head) * D + e;
+            const float2 cs = turn_of(p.positions[node], p.freq.turns[e / 2]);
+            const float a = to_float<T>(at[0]), b = to_float<T>(at[1]);
+            x = (a * cs.x - b * cs.y) * (p.scale * kLog2e);
+            y = (a * cs.y + b * cs.x) * (p.scale * kLog2e);
+        }
+        q_s[r * stride + e] = x;
+        q_s[r * stride + e + 1] = y;
+    }
+    if (tid < kRows) {
+        m_s[tid] = -INFINITY;
+        l_s[tid] = 0.f;
+    }
+    const int rg = tid >> 4, cg = tid & 15;  // rows rg * 4 .. + 3; tokens cg, cg + 16; dims cg * 4 and cg * 4 + 64
+    float acc[4][8];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[r][e] = 0.f;
+
+    for (int t0 = begin; t0 < end; t0 += kTokens) {
+        __syncthreads();
+        if (tid < kTokens) {
+            const int t = t0 + tid;
+            int64_t row = -1;
+            if (t < end) {
+                const int page = p.page_tables[(int64_t)seq * p.max_pages + t / p.page_size];
+                if ((unsigned)page < (unsigned)p.physical_pages) {
+                    row = (int64_t)page * p.page_size + t % p.page_size;
+                } else {  // never read: its tokens are left out and the call is flagged
+                    p.status->code = FLAT_ERR_PAGE_OUT_OF_RANGE;
+                    p.status->where = seq;
+                }
+            }
+            row_s[tid] = row;
+        }
+        __syncthreads();
+        for (int i = tid; i < kTokens * D4; i += kThreads) {
+            const int t = i / D4, e = i % D4;
+            const int64_t row = row_s[t];
+            float k = 0.f, v = 0.f;
+            if (row >= 0 && e < D) {
+                const int64_t at = (row * p.kv_heads + kv_head) * D + e;
+                k = to_float<T>(static_cast<const T *>(p.k)[at]);
+                v = to_float<T>(static_cast<const T *>(p.v)[at]);
+            }
+            k_s[t * stride + e] = k;
+            v_s[t * stride + e] = v;
+        }
+        __syncthreads();
+        float x[4][2];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r][0] = x[r][1] = 0.f;
+        for (int e = 0; e < D4; e += 4) {
+            const float4 k0 = *reinterpret_cast<const float4 *>(k_s + cg * stride + e);
+            const float4 k1 = *reinterpret_cast<const float4 *>(k_s + (cg + 16) * stride + e);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float4 q = *reinterpret_cast<const float4 *>(q_s + (rg * 4 + r) * stride + e);
+                x[r][0] = fmaf(q.x, k0.x, fmaf(q.y, k0.y, fmaf(q.z, k0.z, fmaf(q.w, k0.w, x[r][0]))));
+                x[r][1] = fmaf(q.x, k1.x, fmaf(q.y, k1.y, fmaf(q.z, k1.z, fmaf(q.w, k1.w, x[r][1]))));
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = rg * 4 + r, node = (row0 + row) / p.group;
+            bool on[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int t = cg + 16 * c;
+                on[c] = row < rows && row_s[t] >= 0 && sees(p, s, node, t0 + t);
+                if (!on[c]) x[r][c] = -INFINITY;
+            }
+            float top = fmaxf(x[r][0], x[r][1]);
+#pragma unroll
+            for (int w = 8; w >= 1; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            const float before = m_s[row], now = fmaxf(before, top), base = now == -INFINITY ? 0.f : now;
+            float sum = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const float w = exp2f(x[r][c] - base);
+                p_s[row * (kTokens + 1) + cg + 16 * c] = on[c] ? w : kMasked;
+                if (on[c]) sum += w;
+            }
+#pragma unroll
+            for (int w = 8; w >= 1; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+            __syncwarp();
+            if (cg == 0) {
+                const float a = exp2f(before - base);  // before = -inf gives 0
+                m_s[row] = now;
+                l_s[row] = l_s[row] * a + sum;
+                a_s[row] = a;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float a = a_s[rg * 4 + r];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[r][e] *= a;
+        }
+        for (int t = 0; t < kTokens; ++t) {
+            float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
+            if (cg * 4 < D4) v0 = *reinterpret_cast<const float4 *>(v_s + t * stride + cg * 4);
+            if (cg * 4 + 64 < D4) v1 = *reinterpret_cast<const float4 *>(v_s + t * stride + cg * 4 + 64);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float w = p_s[(rg * 4 + r) * (kTokens + 1) + t];
+                if (w < 0.f) continue;
+                acc[r][0] = fmaf(w, v0.x, acc[r][0]);
+                acc[r][1] = fmaf(w, v0.y, acc[r][1]);
+                acc[r][2] = fmaf(w, v0.z, acc[r][2]);
+                acc[r][3] = fmaf(w, v0.w, acc[r][3]);
+                acc[r][4] = fmaf(w, v1.x, acc[r][4]);
+                acc[r][5] = fmaf(w, v1.y, acc[r][5]);
+                acc[r][6] = fmaf(w, v1.z, acc[r][6]);
+                acc[r][7] = fmaf(w, v1.w, acc[r][7]);
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int row = rg * 4 + r;
+        if (row >= rows) continue;
+        const float m = m_s[row], l = l_s[row];
+        const bool empty = l == 0.f;  // a NaN counts
+        const float inv = empty ? 0.f : 1.0f / l, lse = empty ? -INFINITY : (m + log2f(l)) * kLn2;
+        const int64_t out = (int64_t)(s.first + (row0 + row) / p.group) * p.q_heads + kv_head * p.group + (row0 + row) % p.group;
+        const int64_t part = (int64_t)split * p.max_q * p.q_heads + out;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int d = cg * 4 + (e & 3) + (e >> 2) * 64;
+            if (d >= D) continue;
+            const float o = empty ? 0.f : acc[r][e] * inv;
+            if (p.splits > 1) p.partial_o[part * D + d] = o;
+            else static_cast<T *>(p.o)[out * D + d] = from_float<T>(o);
+        }
+        if (cg == 0) (p.splits > 1 ? p.partial_lse[part] : p.lse[out]) = lse;
+    }
+}
+
+// Joins the chunks of the rows of one sequence's drafted token: LSE = log sum exp(LSE_i), O = sum exp(LSE_i - LSE) O_i, in chunk order.
+template <typename T> __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__ TreeParams p) {
+    grid_dependency_wait();
+    grid_dependency_launch();
+    const int seq = blockIdx.z, node = blockIdx.y;
+    const Span s = span_of(p, seq);
+    if (node >= s.nodes) return;
+    const int parts = max(1, (s.tokens + p.chunk - 1) / p.chunk), D = p.head_dim;
+    const int64_t rows = (int64_t)p.max_q * p.q_heads;
+    for (int head = blockIdx.x * 4 + (threadIdx.x >> 5); head < p.q_heads; head += gridDim.x * 4) {
+        const int64_t row = (int64_t)(s.first + node) * p.q_heads + head;
+        float mx = -INFINITY, sum = 0.f;
+        for (int i = 0; i < parts; ++i) mx = fmaxf(mx, p.partial_lse[i * rows + row]);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        for (int i = 0; i < parts; ++i) sum += expf(p.partial_lse[i * rows + row] - base);
+        const bool empty = sum == 0.f;
+        const float total = empty ? -INFINITY : base + logf(sum);
+        for (int d = threadIdx.x & 31; d < D; d += 32) {
+            float o = 0.f;
+            for (int i = 0; i < parts; ++i) {
+                const float w = empty ? 0.f : expf(p.partial_lse[i * rows + row] - total);
+                o = fmaf(w, p.partial_o[(i * rows + row) * D + d], o);
+            }
+            static_cast<T *>(p.o)[row * D + d] = from_float<T>(o);
+        }
+        if ((threadIdx.x & 31) == 0) p.lse[row] = total;
+    }
+}
+
+template <typename T> int launch(flat_ctx *ctx, TreeParams &p) {
+    const int tiles = (int)(((int64_t)p.max_nodes * p.group + kRows - 1) / kRows);
+    if ((int64_t)tiles * p.kv_heads > 65535)
+        return fail(ctx, FLAT_ERR_DISPATCH_LIMIT, "%d drafted tokens of %d heads are more row tiles than one launch has", p.max_nodes, p.q_heads);
+    // chunks of the longest context that fill the device about four times, 128 tokens at least, as many as the scratch holds
+    const int64_t rows = (int64_t)p.max_q * p.q_heads, units = (int64_t)tiles * p.kv_heads * p.num_seqs;
+    const int64_t fit = (int64_t)((kPagedScratchBytes - kPagedPlanBytes) / (rows * (p.head_dim + 1) * sizeof(float)));
+    int64_t splits = std::min<int64_t>({(p.max_context + 127) / 128, std::max<int64_t>(1, (int64_t)ctx->sm_count * 8 / units), 256, fit});
+    if (splits < 1) splits = 1;
+    p.chunk = (int)((p.max_context + splits - 1) / splits + kTokens - 1) / kTokens * kTokens;
+    p.splits = (int)((p.max_context + p.chunk - 1) / p.chunk);
+    p.partial_o = reinterpret_cast<float *>(static_cast<char *>(ctx->paged_scratch) + kPagedPlanBytes);
+    p.partial_lse = p.partial_o + p.splits * rows * p.head_dim;
+    const int stride = (p.head_dim + 3) / 4 * 4 + 4;
+    const size_t smem = ((kRows + 2 * kTokens) * stride + kRows * (kTokens + 1) + 3 * kRows) * sizeof(float);
+    static_assert((32 + 64) * (kMaxHeadDim + 4) * 4 + 32 * 33 * 4 + 96 * 4 < 64 << 10, "shared memory of the largest head_dim");
+    FLAT_CUDA_OK(ctx, cudaFuncSetAttribute(tree_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 << 10));
+    {
+        KernelTimer timer(ctx);
+        FLAT_CUDA_OK(ctx, launch_dependent(may_overlap_previous(ctx), tree_simt_kernel<T>, dim3((unsigned)p.splits, (unsigned)(tiles * p.kv_heads), (unsigned)p.num_seqs),
+                                           kThreads, smem, ctx->stream, p));
+    }
+    ctx->launches += 1;
+    if (p.splits > 1) {
+        FLAT_CUDA_OK(ctx, launch_dependent(true, tree_merge_kernel<T>, dim3((unsigned)((p.q_heads + 3) / 4), (unsigned)p.max_nodes, (unsigned)p.num_seqs), 128, 0,
+                                           ctx->stream, p));
+        ctx->launches += 1;
+    }
+    return FLAT_OK;
+}
+
+}  // namespace
+
+int launch_tree_simt(flat_ctx *ctx, int dtype, TreeParams &p) { return dtype == FLAT_BF16 ? launch<__nv_bfloat16>(ctx, p) : launch<float>(ctx, p); }
+
+}  // namespace flat

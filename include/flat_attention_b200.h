@@ -612,6 +612,91 @@ int32_t flat_splitkv_merge(flat_ctx *ctx, int32_t dtype, uint64_t parts, uint64_
                            uint64_t head_dim, flat_buffer partial_o, flat_buffer partial_lse,
                            flat_buffer out_and_lse);
 
+/* ---- batches whose lengths and page tables stay on the device -------------------------- */
+
+/* The five calls of a serving step that verifies drafted tokens: pages and slots for them (reserve), their K/V rows
+ * (write), their attention (tree), the rows of the accepted ones (accept), the pages that are not needed any more
+ * (release).  Lengths, tables and counts are device arrays that no call reads on the host, so that a step can be
+ * captured in a CUDA graph and replayed; the host gives upper bounds.  All of them enqueue on the context's stream.
+ * Their scratch (48 MiB) is allocated by the first of them that is made on a context and never moves: make one call
+ * before a stream capture.  It is used in stream order, so graphs captured on one context must not run at the same
+ * time; two contexts have nothing in common.  What the host cannot see is checked on the device: a sequence whose
+ * entries make no sense is left out (as each call says) and flat_ctx_device_status reports it.  No counterpart in the
+ * reference, whose paged caches hold one sequence and whose page table is host data (src/paged_kv.rs:75-188). */
+typedef struct flat_paged_batch {
+    uint64_t num_seqs;          /* at most 65535 */
+    uint64_t page_size;         /* tokens of a page */
+    uint64_t physical_pages;    /* pages of the pool; page_size * physical_pages < 2^31 */
+    uint64_t max_pages_per_seq; /* row length of page_tables */
+    int32_t *page_tables;       /* DEVICE [num_seqs, max_pages_per_seq]: entries at and behind page_counts are not read */
+    int32_t *page_counts;       /* DEVICE [num_seqs]: pages that a sequence holds */
+    int32_t *context_lens;      /* DEVICE [num_seqs]: live tokens, drafted ones not among them */
+    int32_t *free_pages;        /* DEVICE [physical_pages]: a stack of free pages, its top at free_count - 1 */
+    int32_t *free_count;        /* DEVICE [1] */
+} flat_paged_batch;
+
+/* Pages and slots for new_lens[s] tokens behind the live ones of each sequence.  Sequence s needs
+ *   need[s] = max(0, ceil((context_lens[s] + new_lens[s]) / page_size) - page_counts[s])
+ * pages; they are taken from the top of the stack in sequence order and entered in page_tables.  It gets them all or, where
+ * the stack ends before, none (sequences that need no page are served all the same).  The new tokens are packed sequence by
+ * sequence: new_offsets [num_seqs + 1] receives where each sequence's start, slot_map [max_new_tokens] the row of the pool
+ * of each and positions [max_new_tokens] its position, context_lens[s] + i for the i-th or, with depths (optional,
+ * [max_new_tokens], packed alike), context_lens[s] + depths[token].  Tokens of a sequence that is refused, and entries behind the
+ * last token, get slot -1 and position 0.  page_counts_out [num_seqs], free_count_out [1] (null: in place) receive the
+ * counts afterwards, context_lens_out (null: not written; may be context_lens) context_lens + new_lens of served sequences.
+ * Device status: CAPACITY_EXCEEDED (a sequence was refused for want of pages), INVALID_CACHE_LENGTH (negative lengths, more
+ * live tokens than its pages hold, more than max_pages_per_seq pages or more than max_new_tokens tokens),
+ * PAGE_OUT_OF_RANGE (an entry outside the pool; its tokens get slot -1), CAPACITY_OVERFLOW (free_count outside the pool). */
+int32_t flat_paged_batch_reserve(flat_ctx *ctx, const flat_paged_batch *batch, const int32_t *new_lens_dev,
+                                 const int32_t *depths_dev, uint64_t max_new_tokens, int32_t *page_counts_out,
+                                 int32_t *free_count_out, int32_t *context_lens_out, int32_t *new_offsets_dev,
+                                 int32_t *slot_map_dev, int32_t *positions_dev);
+
+/* Gives back the pages of each sequence behind its first keep_lens[s] tokens (0: all of them): page_counts[s] becomes
+ * min(page_counts[s], ceil(keep_lens[s] / page_size)), and the pages go on the stack in sequence order, a sequence's last page
+ * first.  page_tables keeps its entries (those at and behind page_counts mean nothing).  page_counts_out, free_count_out
+ * as above.  Device status: INVALID_CACHE_LENGTH (negative length or count: the sequence keeps its pages), CAPACITY_OVERFLOW
+ * (more pages than the pool has: the rest is dropped), PAGE_OUT_OF_RANGE (an entry outside the pool is on the stack now). */
+int32_t flat_paged_batch_release(flat_ctx *ctx, const flat_paged_batch *batch, const int32_t *keep_lens_dev,
+                                 int32_t *page_counts_out, int32_t *free_count_out);
+
+/* Rows of new tokens into a pool: K row t, turned at positions[t] (null: stored as it is), and V row t go to row slot_map[t]
+ * of K and V [pool_rows, kv_heads*head_dim].  Sources are [tokens, kv_heads*head_dim]; f32 or bf16.  A negative slot leaves the
+ * token out, one at or behind pool_rows too (device status PAGE_OUT_OF_RANGE).  Slots have to differ: what a row holds
+ * that is named twice is unspecified.  Angles are position * theta^(-2j/head_dim) to 2^-32 of a turn at any position
+ * (the single-sequence append forms them as 32-bit floats, like the reference: the two differ by position * 2^-25 radians
+ * in the fastest pair). */
+int32_t flat_paged_kv_write(flat_ctx *ctx, int32_t dtype, uint64_t tokens, uint64_t kv_heads, uint64_t head_dim,
+                            uint64_t pool_rows, const int32_t *slot_map_dev, const int32_t *positions_dev, float theta,
+                            flat_buffer k_source, flat_buffer v_source, flat_buffer k, flat_buffer v);
+
+/* Attention of drafted tokens over the cache.  The drafted tokens of sequence s are rows q_offsets[s] .. q_offsets[s+1] - 1 of Q
+ * [max_q_tokens, q_heads*head_dim] (as flat_paged_batch_reserve packs them), and their K/V rows are already in the cache behind its
+ * context_lens[s] live tokens.  Drafted token i sees all live tokens, and drafted token j of its sequence iff bit j % 32 of
+ * tree_mask[i, j / 32] is set (DEVICE [max_q_tokens, mask_words]; each token's own bit is set like its ancestors').  Without
+ * tree_mask (null) config->causal decides: 1 a chain (j <= i), 0 all see one another.  One token a sequence is plain
+ * decode with all lengths on the device.  Q is raw and turned at q_positions, K is turned already, scale as elsewhere.
+ * max_nodes bounds the drafted tokens of a sequence and max_context its live and drafted tokens together.  Output packed
+ * [O(max_q_tokens*q_heads*head_dim) | LSE(max_q_tokens*q_heads)] (flat_decode_layout_for with batch = max_q_tokens); rows behind
+ * q_offsets[num_seqs] are left as they are.  A token that sees nothing gets O = 0, LSE = -inf.  K and V of tokens that a row does not
+ * see have no influence on it, NaN and infinities among them.  Results are bitwise repeatable for the same lengths and bounds.
+ * Device status: LENGTH_MISMATCH (offsets that fall or leave Q, more than max_nodes drafted tokens, a negative length: the
+ * sequence's rows are not written), PAGE_OUT_OF_RANGE (tokens without a page of the pool, or behind max_context: left out). */
+int32_t flat_decode_paged_tree(flat_ctx *ctx, int32_t dtype, const flat_paged_batch *batch, uint64_t q_heads,
+                               uint64_t kv_heads, uint64_t head_dim, uint64_t max_q_tokens, uint64_t max_nodes,
+                               uint64_t max_context, const int32_t *q_offsets_dev, const int32_t *q_positions_dev,
+                               const int32_t *tree_mask_dev, uint64_t mask_words, const flat_attention_config *config,
+                               float theta, flat_buffer q, flat_buffer k, flat_buffer v, flat_buffer out_and_lse);
+
+/* Keeps one path of each sequence's drafted tokens: accept_nodes [num_seqs, max_accept] names them, strictly rising, the first
+ * accept_lens[s] of each row count; the K/V row of the j-th moves to the j-th place behind the live tokens, in place, and
+ * context_lens_out[s] (null: in place) becomes context_lens[s] + accept_lens[s].  Rotations stay right where a token's position is its
+ * place in the path, as for a tree whose depths were given to flat_paged_batch_reserve.  A sequence whose path does not
+ * rise, is longer than max_accept or leaves its pages moves nothing and keeps its length (device status LENGTH_MISMATCH). */
+int32_t flat_paged_kv_accept(flat_ctx *ctx, int32_t dtype, const flat_paged_batch *batch, uint64_t kv_heads,
+                             uint64_t head_dim, uint64_t max_accept, const int32_t *accept_nodes_dev,
+                             const int32_t *accept_lens_dev, int32_t *context_lens_out, flat_buffer k, flat_buffer v);
+
 /* ---- chunked prefill ----------------------------------------------------------------- */
 
 /* WgpuChunkedProjectionPrefillPipeline::encode (src/wgpu_chunked_prefill.rs:156-299):

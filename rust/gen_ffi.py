@@ -22,7 +22,8 @@ STRUCTS = {"flat_attention_shape": "FlatAttentionShape", "flat_attention_config"
            "flat_varlen_sequence": "FlatVarlenSequence", "flat_paged_kv_telemetry": "FlatPagedKvTelemetry",
            "flat_paged_kv_address": "FlatPagedKvAddress", "flat_numerical_guarantees": "FlatNumericalGuarantees",
            "flat_device_fingerprint": "FlatDeviceFingerprint", "flat_device_capabilities": "FlatDeviceCapabilities",
-           "flat_dispatch_telemetry": "FlatDispatchTelemetry", "flat_benchmark_manifest": "FlatBenchmarkManifest"}
+           "flat_dispatch_telemetry": "FlatDispatchTelemetry", "flat_paged_batch": "FlatPagedBatch",
+           "flat_benchmark_manifest": "FlatBenchmarkManifest"}
 OPAQUE = {"flat_ctx": "FlatCtx", "flat_paged_kv_table": "FlatPagedKvTable", "flat_paged_kv_cache": "FlatPagedKvCache",
           "flat_resident_kv_cache": "FlatResidentKvCache", "flat_prepared_forward": "FlatPreparedForward",
           "flat_prepared_backward": "FlatPreparedBackward", "flat_splitkv_exchange": "FlatSplitKvExchange"}

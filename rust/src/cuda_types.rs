@@ -113,6 +113,21 @@ pub struct FlatPagedKvTelemetry {
     pub generation: u64,
 }
 
+/// A batch of sequences whose lengths and page tables stay on the device; the pointers are device arrays of `i32`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct FlatPagedBatch {
+    pub num_seqs: u64,
+    pub page_size: u64,
+    pub physical_pages: u64,
+    pub max_pages_per_seq: u64,
+    pub page_tables: *mut i32,
+    pub page_counts: *mut i32,
+    pub context_lens: *mut i32,
+    pub free_pages: *mut i32,
+    pub free_count: *mut i32,
+}
+
 #[repr(C)]
 #[derive(Clone, Copy, Debug, Default, PartialEq, Eq)]
 pub struct FlatPagedKvAddress {
