@@ -9,6 +9,7 @@
 // read once per 32 rows.  A masked token counts for nothing whatever its K and V hold: its score is replaced, not added to, and its
 // product with V is left out rather than formed with weight 0.
 #include "common.h"
+#include "tree.cuh"
 #include "turns.cuh"
 
 namespace flat {
@@ -25,40 +26,14 @@ template <typename T> __device__ __forceinline__ T from_float(float x);
 template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// What a block knows of its sequence.  The device arrays hold whatever they hold: the rows stay inside q and o, the tokens inside
-// the pages that the sequence holds.
-struct Span {
-    int first, nodes, len, tokens;  // rows of q; drafted tokens; live tokens; tokens that there are pages for
-};
-__device__ __forceinline__ Span span_of(const TreeParams &p, int seq) {
-    Span s;
-    s.first = p.q_offsets[seq];
-    s.nodes = p.q_offsets[seq + 1] - s.first;
-    s.len = p.context_lens[seq];
-    if (s.first < 0 || s.nodes <= 0 || s.nodes > p.max_nodes || s.nodes > p.max_q - s.first || s.len < 0) {
-        if (s.nodes != 0 && threadIdx.x == 0) {
-            p.status->code = FLAT_ERR_LENGTH_MISMATCH;
-            p.status->where = seq;
-        }
-        s.nodes = 0;
-        s.tokens = 0;
-        return s;
-    }
-    const int64_t room = (int64_t)min(max(p.page_counts[seq], 0), p.max_pages) * p.page_size, want = (int64_t)s.len + s.nodes;
-    s.tokens = (int)min(min(want, room), (int64_t)p.max_context);
-    if (s.tokens < want && threadIdx.x == 0) {
-        p.status->code = FLAT_ERR_PAGE_OUT_OF_RANGE;
-        p.status->where = seq;
-    }
+__device__ __forceinline__ TreeSequence span_of(const TreeParams &p, int seq) {
+    const TreeSequence s = tree_sequence(p, seq);
+    if (s.code && threadIdx.x == 0) tree_report(p, s.code, seq);
     return s;
 }
 
-__device__ __forceinline__ bool sees(const TreeParams &p, const Span &s, int node, int token) {
-    if (token < s.len) return true;
-    const int j = token - s.len;
-    if (j >= s.nodes) return false;
-    if (!p.mask) return !p.causal || j <= node;
-    return (p.mask[(int64_t)(s.first + node) * p.mask_words + (j >> 5)] >> (j & 31)) & 1u;
+__device__ __forceinline__ bool sees(const TreeParams &p, const TreeSequence &s, int node, int token) {
+    return token < s.len || (token - s.len < s.nodes && tree_sees(p, s, node, token - s.len));
 }
 
 template <typename T> __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_constant__ TreeParams p) {
@@ -72,7 +47,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) tree_simt_kern
     __shared__ int64_t row_s[kTokens];
     const int tiles = (p.max_nodes * p.group + kRows - 1) / kRows;
     const int seq = blockIdx.z, kv_head = blockIdx.y / tiles, row0 = blockIdx.y % tiles * kRows, split = blockIdx.x;
-    const Span s = span_of(p, seq);
+    const TreeSequence s = span_of(p, seq);
     const int rows = min(kRows, s.nodes * p.group - row0);
     if (rows <= 0) return;
     const int begin = (int)min((int64_t)split * p.chunk, (int64_t)s.tokens), end = (int)min((int64_t)begin + p.chunk, (int64_t)s.tokens);
@@ -231,7 +206,7 @@ template <typename T> __global__ void __launch_bounds__(128) tree_merge_kernel(c
     grid_dependency_wait();
     grid_dependency_launch();
     const int seq = blockIdx.z, node = blockIdx.y;
-    const Span s = span_of(p, seq);
+    const TreeSequence s = span_of(p, seq);
     if (node >= s.nodes) return;
     const int parts = max(1, (s.tokens + p.chunk - 1) / p.chunk), D = p.head_dim;
     const int64_t rows = (int64_t)p.max_q * p.q_heads;
