@@ -34,6 +34,12 @@ __device__ __forceinline__ float2 turn_of(int32_t position, uint64_t turns) {
     sincospif((float)(int32_t)(phase >> 32) * 0x1p-31f, &cs.y, &cs.x);
     return cs;
 }
+// The same by the special-function unit: 2^-21 off at most, for queries that are rounded to 16 bits in two summands anyway
+__device__ __forceinline__ float2 turn_of_fast(int32_t position, uint64_t turns) {
+    const uint64_t phase = turns * (uint64_t)(int64_t)position + 0x80000000ull;
+    const float angle = (float)(int32_t)(phase >> 32) * (0x1p-31f * 3.14159265358979f);
+    return make_float2(__cosf(angle), __sinf(angle));
+}
 #endif
 
 }  // namespace flat
