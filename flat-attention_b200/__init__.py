@@ -163,9 +163,15 @@ def lib() -> C.CDLL:
     return _lib
 
 
+_torch_module = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
 
 
 def buf(t) -> Buffer:
@@ -497,10 +503,10 @@ class Context:
         k_source / v_source [tokens, kv_heads*head_dim], k / v [pool_rows, kv_heads*head_dim]."""
         tokens = slot_map.numel()
         _ints(tokens, slot_map=slot_map, positions=positions)
-        _same_type(k_source, v_source, k, v)
-        pool_rows = _b(k).bytes // (kv_heads * head_dim * k_source.element_size()) if kv_heads * head_dim else 0
-        self.check(lib().flat_paged_kv_write(self.h, _dtype_of(k_source), tokens, kv_heads, head_dim, pool_rows, _p(slot_map), _p(positions),
-                                             theta, _whole(k_source), _whole(v_source), _whole(k), _whole(v)))
+        dtype, pool = _same_type(k_source, v_source, k, v), _whole(k)
+        pool_rows = pool.bytes // (kv_heads * head_dim * k_source.element_size()) if kv_heads * head_dim else 0
+        self.check(lib().flat_paged_kv_write(self.h, dtype, tokens, kv_heads, head_dim, pool_rows, _p(slot_map), _p(positions),
+                                             theta, _whole(k_source), _whole(v_source), pool, _whole(v)))
 
     def decode_paged_tree(self, batch: "PagedBatch", q_heads: int, kv_heads: int, head_dim: int, max_nodes: int, max_context: int, q_offsets,
                           q_positions, tree_mask, cfg, theta: float, q, k, v, out):
@@ -516,8 +522,7 @@ class Context:
                 raise FlatAttentionError(7, f"tree_mask has shape {tuple(tree_mask.shape)}, expected [{tokens}, words]")
             words = tree_mask.shape[1]
             _ints(tokens * words, tree_mask=tree_mask)
-        _same_type(q, k, v)
-        self.check(lib().flat_decode_paged_tree(self.h, _dtype_of(q), batch.ref, q_heads, kv_heads, head_dim, tokens, max_nodes, max_context,
+        self.check(lib().flat_decode_paged_tree(self.h, _same_type(q, k, v), batch.ref, q_heads, kv_heads, head_dim, tokens, max_nodes, max_context,
                                                 _p(q_offsets), _p(q_positions), _p(tree_mask), words, C.byref(cfg), theta, _whole(q), _whole(k),
                                                 _whole(v), _whole(out)))
 
@@ -639,28 +644,29 @@ def _p(t):
 
 def _ints(elements: int, **tensors):
     """Each given tensor is a contiguous int32 CUDA tensor of at least `elements`."""
+    int32 = _torch().int32
     for name, t in tensors.items():
-        if t is None:
+        if t is None or (t.dtype is int32 and t.is_cuda and t.is_contiguous() and t.numel() >= elements):
             continue
-        if t.dtype != _torch().int32:
+        if t.dtype is not int32:
             raise FlatAttentionError(26, f"{name} must be int32, is {t.dtype}")
         if not t.is_cuda or not t.is_contiguous():
             raise FlatAttentionError(29, f"{name} must be a contiguous CUDA tensor")
-        if t.numel() < elements:
-            raise FlatAttentionError(22, f"{name} has {t.numel()} elements, requires {elements}")
+        raise FlatAttentionError(22, f"{name} has {t.numel()} elements, requires {elements}")
 
 
 def _same_type(*tensors):
     """Tensors (flat_buffer views have no type) share one; returns its dtype code, None if all are views."""
-    code = None
+    first = None
     for t in tensors:
         if isinstance(t, Buffer):
             continue
-        c = _dtype_of(t)
-        if code is not None and c != code:
+        if first is None:
+            first = t.dtype
+            code = _dtype_of(t)
+        elif t.dtype is not first:
             raise FlatAttentionError(26, "Q, K and V differ in type")
-        code = c
-    return code
+    return None if first is None else code
 
 
 def _whole(x) -> Buffer:
@@ -669,7 +675,7 @@ def _whole(x) -> Buffer:
         return x
     if not x.is_cuda or not x.is_contiguous():
         raise FlatAttentionError(29, "tensors must be contiguous and on the device")
-    return buf(x)
+    return Buffer(x.data_ptr(), x.nbytes)
 
 
 class PagedBatch:

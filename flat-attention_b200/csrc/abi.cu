@@ -53,7 +53,11 @@ int ensure_paged_scratch(flat_ctx *ctx) {
     if (capture != cudaStreamCaptureStatusNone)
         return fail(ctx, FLAT_ERR_EXECUTION, "the first call on a device-resident batch allocates its scratch: make one before the capture");
     cudaError_t e = cudaMalloc(&ctx->paged_scratch, kPagedScratchBytes);
-    if (e == cudaSuccess) return FLAT_OK;
+    if (e == cudaSuccess) {
+        e = cudaMemsetAsync(ctx->paged_scratch, 0, kPagedPlanBytes, ctx->stream);  // the tickets
+        if (e == cudaSuccess) return FLAT_OK;
+        cudaFree(ctx->paged_scratch);
+    }
     cudaGetLastError();
     ctx->paged_scratch = nullptr;
     return fail(ctx, FLAT_ERR_EXECUTION, "cudaMalloc of %llu bytes failed: %s", (unsigned long long)kPagedScratchBytes, cudaGetErrorString(e));
@@ -1845,7 +1849,8 @@ PagedBatchParams batch_params(flat_ctx *ctx, const flat_paged_batch *b) {
     p.plan = static_cast<int4 *>(ctx->paged_scratch);
     p.plan_offsets = reinterpret_cast<int32_t *>(p.plan + kMaxBatchSeqs + 1);
     p.plan_free_count = p.plan_offsets + kMaxBatchSeqs + 1;
-    static_assert((kMaxBatchSeqs + 1) * (sizeof(int4) + sizeof(int32_t)) + sizeof(int32_t) <= kPagedPlanBytes, "plan region");
+    p.plan_ticket = reinterpret_cast<unsigned *>(p.plan_free_count + 1);
+    static_assert((kMaxBatchSeqs + 1) * (sizeof(int4) + sizeof(int32_t)) + 2 * sizeof(int32_t) <= kPagedPlanBytes, "plan region");
     return p;
 }
 
@@ -1993,6 +1998,9 @@ int32_t flat_decode_paged_tree(flat_ctx *ctx, int32_t dtype, const flat_paged_ba
     if (tree_mask_dev && (max_nodes > 32 * std::min<uint64_t>(mask_words, 2048) || mask_words > 2048))
         return fail(ctx, FLAT_ERR_LENGTH_MISMATCH, "tree_mask rows of %llu words do not hold %llu drafted tokens", (unsigned long long)mask_words,
                     (unsigned long long)max_nodes);
+    if (max_nodes * (q_heads / kv_heads) > (uint64_t)1 << 24)
+        return fail(ctx, FLAT_ERR_DISPATCH_LIMIT, "%llu drafted tokens of %llu heads a group are too many rows", (unsigned long long)max_nodes,
+                    (unsigned long long)(q_heads / kv_heads));
     if ((st = resolve_scale(ctx, config, head_dim, &scale))) return st;
     if ((st = validate_rows(ctx, dtype, batch->page_size * batch->physical_pages, kv_heads, head_dim, k, v, &row))) return st;
     flat_decode_layout layout;

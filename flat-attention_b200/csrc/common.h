@@ -328,8 +328,8 @@ struct PagedBatchParams {
     int4 *plan;             // scratch, per sequence.  reserve: live tokens, held pages, pages given before, granted; release: -, held pages, pages left, -
     int32_t *plan_offsets;  // scratch, release: where each sequence's pages go, [num_seqs + 1]
     int32_t *plan_free_count;
+    unsigned *plan_ticket;  // scratch: 0 between calls
     DeviceStatus *status;
-    int fused;
 };
 int launch_paged_batch(flat_ctx *ctx, PagedBatchParams &p, bool release);
 struct TurnTable {
@@ -369,7 +369,7 @@ struct TreeParams {
     float scale;
     TurnTable freq;
     DeviceStatus *status;
-    int splits, chunk;                  // of the generic kernel
+    int splits, chunk, vectors;         // of the generic kernel
     float *partial_o, *partial_lse;
 };
 int launch_tree_simt(flat_ctx *ctx, int dtype, TreeParams &p);

@@ -144,10 +144,11 @@ __global__ void __launch_bounds__(kThreads) paged_write_pairs_kernel(const __gri
 // Row j of a sequence's drafts := row path[j], j = 0, 1, ...  The path rises strictly, so path[j] >= j: a step's destination is never
 // a later step's source, and what a step overwrites an earlier one has read, if each thread goes through the steps in order.  A
 // block takes a sequence, a thread one 16-byte (otherwise one-element) column of its rows at a time, kFlight rows in flight, so no
-// two threads touch the same bytes.
+// two threads touch the same bytes.  Which rows the steps mean is looked up once for the block, kSteps at a time.
 template <typename V> __global__ void __launch_bounds__(kThreads) paged_accept_kernel(const __grid_constant__ PagedAcceptParams p) {
-    constexpr int kFlight = 8;
+    constexpr int kFlight = 8, kSteps = kThreads;
     __shared__ int bad_s;
+    __shared__ int64_t from_s[kSteps], to_s[kSteps];  // < 0 in from_s: stays
     grid_dependency_wait();
     grid_dependency_launch();
     const int seq = blockIdx.x;
@@ -155,22 +156,25 @@ template <typename V> __global__ void __launch_bounds__(kThreads) paged_accept_k
     const int32_t *path = p.path + (int64_t)seq * p.max_accept;
     const int32_t *table = p.page_tables + (int64_t)seq * p.max_pages;
     auto row_of = [&](int node) -> int64_t {  // < 0: not a row that the sequence holds
-        const int64_t t = (int64_t)len + node, logical = t / p.page_size;
-        if (logical >= held) return -1;
+        const unsigned t = (unsigned)len + (unsigned)node, logical = t / (unsigned)p.page_size;
+        if (node < 0 || (int64_t)logical >= held) return -1;
         const int page = table[logical];
-        return (unsigned)page < (unsigned)p.physical_pages ? (int64_t)page * p.page_size + (t - logical * p.page_size) : -1;
+        return (unsigned)page < (unsigned)p.physical_pages ? (int64_t)page * p.page_size + (t - logical * (unsigned)p.page_size) : -1;
     };
-    // the whole path first: a sequence moves all of it or nothing
     if (threadIdx.x == 0) bad_s = take < 0 || take > p.max_accept || len < 0;
     __syncthreads();
-    if (!bad_s) {
-        bool bad = false;
-        for (int j = threadIdx.x; j < take; j += kThreads) {
-            const int node = path[j];
-            bad |= node < j || (j > 0 && path[j - 1] >= node) || row_of(node) < 0 || row_of(j) < 0;
-        }
-        if (bad) bad_s = 1;
-    }
+    // the whole path first, its beginning last: a sequence moves all of it or nothing
+    auto look = [&](int base) {
+        const int j = base + threadIdx.x;
+        if (j >= take) return;
+        const int node = path[j], before = j > 0 ? path[j - 1] : -1;
+        const int64_t from = row_of(node), to = row_of(j);
+        if (node < j || before >= node || from < 0 || to < 0) bad_s = 1;
+        from_s[threadIdx.x] = node == j ? -1 : from;
+        to_s[threadIdx.x] = to;
+    };
+    if (!bad_s)
+        for (int base = (max(take, 1) - 1) / kSteps * kSteps; base >= 0; base -= kSteps) look(base);
     __syncthreads();
     const bool bad = bad_s != 0;
     if (threadIdx.x == 0) {  // context_lens_out may be context_lens: every thread has read the length
@@ -178,19 +182,27 @@ template <typename V> __global__ void __launch_bounds__(kThreads) paged_accept_k
         if (bad) flag(p.status, FLAT_ERR_LENGTH_MISMATCH, seq);
     }
     if (bad) return;
-    for (int64_t column = threadIdx.x; column < 2 * p.row_vecs; column += kThreads) {
-        V *at = column < p.row_vecs ? static_cast<V *>(p.k) + column : static_cast<V *>(p.v) + (column - p.row_vecs);
-        for (int base = 0; base < take; base += kFlight) {
-            V x[kFlight];
-            bool moves[kFlight];
+    for (int base = 0; base < take; base += kSteps) {
+        if (base > 0) {
+            __syncthreads();
+            look(base);
+            __syncthreads();
+        }
+        const int steps = min(kSteps, take - base);
+        for (int64_t column = threadIdx.x; column < 2 * p.row_vecs; column += kThreads) {
+            V *at = column < p.row_vecs ? static_cast<V *>(p.k) + column : static_cast<V *>(p.v) + (column - p.row_vecs);
+            for (int j = 0; j < steps; j += kFlight) {
+                V x[kFlight];
+                bool moves[kFlight];
 #pragma unroll
-            for (int u = 0; u < kFlight; ++u) {
-                moves[u] = base + u < take && path[base + u] != base + u;
-                if (moves[u]) x[u] = at[row_of(path[base + u]) * p.row_vecs];
+                for (int u = 0; u < kFlight; ++u) {
+                    moves[u] = j + u < steps && from_s[j + u] >= 0;
+                    if (moves[u]) x[u] = at[from_s[j + u] * p.row_vecs];
+                }
+#pragma unroll
+                for (int u = 0; u < kFlight; ++u)
+                    if (moves[u]) at[to_s[j + u] * p.row_vecs] = x[u];
             }
-#pragma unroll
-            for (int u = 0; u < kFlight; ++u)
-                if (moves[u]) at[row_of(base + u) * p.row_vecs] = x[u];
         }
     }
 }

@@ -16,7 +16,7 @@ namespace flat {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kRows = 32, kTokens = 32, kThreads = 128;
+constexpr int kRows = 32, kTokens = 32, kThreads = 128, kMaxSplits = 256;
 constexpr float kMasked = -1.f;  // in place of a weight, which is never negative
 
 template <typename T> __device__ __forceinline__ float to_float(T x);
@@ -25,6 +25,21 @@ template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat
 template <typename T> __device__ __forceinline__ T from_float(float x);
 template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Four values from `at` on as f32, `left` of them there; vec: rows are whole aligned groups of four.
+template <typename T> __device__ __forceinline__ float4 load4(const T *at, bool vec, int left);
+template <> __device__ __forceinline__ float4 load4<float>(const float *at, bool vec, int left) {
+    if (vec) return *reinterpret_cast<const float4 *>(at);
+    return make_float4(at[0], left > 1 ? at[1] : 0.f, left > 2 ? at[2] : 0.f, left > 3 ? at[3] : 0.f);
+}
+template <> __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16 *at, bool vec, int left) {
+    if (vec) {
+        const uint2 x = *reinterpret_cast<const uint2 *>(at);
+        return make_float4(__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u), __uint_as_float(x.y << 16), __uint_as_float(x.y & 0xffff0000u));
+    }
+    return make_float4(to_float<__nv_bfloat16>(at[0]), left > 1 ? to_float<__nv_bfloat16>(at[1]) : 0.f, left > 2 ? to_float<__nv_bfloat16>(at[2]) : 0.f,
+                       left > 3 ? to_float<__nv_bfloat16>(at[3]) : 0.f);
+}
 
 __device__ __forceinline__ TreeSequence span_of(const TreeParams &p, int seq) {
     const TreeSequence s = tree_sequence(p, seq);
@@ -54,25 +69,31 @@ template <typename T> __global__ void __launch_bounds__(kThreads) tree_simt_kern
     if (begin >= end && split > 0) return;  // the merge leaves it out
 
     // the rows' queries, turned, with the softmax scale and log2(e): scores come out in the exp2 domain
-    for (int i = tid; i < kRows * (stride / 2); i += kThreads) {
-        const int r = i / (stride / 2), e = i % (stride / 2) * 2;
-        float x = 0.f, y = 0.f;
-        if (r < rows && e < D) {
-            const int node = s.first + (row0 + r) / p.group, head = kv_head * p.group + (row0 + r) % p.group;
-            const T *at = static_cast<const T *>(p.q) + ((int64_t)node * p.q_heads + head) * D + e;
-            const float2 cs = turn_of(p.positions[node], p.freq.turns[e / 2]);
-            const float a = to_float<T>(at[0]), b = to_float<T>(at[1]);
-            x = (a * cs.x - b * cs.y) * (p.scale * kLog2e);
-            y = (a * cs.y + b * cs.x) * (p.scale * kLog2e);
+    const int rg = tid >> 4, cg = tid & 15;  // rows rg * 4 .. + 3; tokens cg, cg + 16; dims cg * 4 and cg * 4 + 64
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int e = cg * 4 + h * 64;
+        if (e >= D4) break;
+#pragma unroll
+        for (int i = 0; i < kRows / 8; ++i) {
+            const int r = rg + 8 * i;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows) {
+                const int node = s.first + (row0 + r) / p.group, head = kv_head * p.group + (row0 + r) % p.group;
+                const float4 q = load4<T>(static_cast<const T *>(p.q) + ((int64_t)node * p.q_heads + head) * D + e, p.vectors, D - e);
+                const int position = p.positions[node];
+                const float scale = p.scale * kLog2e;
+                const float2 c0 = turn_of(position, p.freq.turns[e / 2]), c1 = e + 2 < D ? turn_of(position, p.freq.turns[e / 2 + 1]) : make_float2(0.f, 0.f);
+                x = make_float4((q.x * c0.x - q.y * c0.y) * scale, (q.x * c0.y + q.y * c0.x) * scale, (q.z * c1.x - q.w * c1.y) * scale,
+                                (q.z * c1.y + q.w * c1.x) * scale);
+            }
+            *reinterpret_cast<float4 *>(q_s + r * stride + e) = x;
         }
-        q_s[r * stride + e] = x;
-        q_s[r * stride + e + 1] = y;
     }
     if (tid < kRows) {
         m_s[tid] = -INFINITY;
         l_s[tid] = 0.f;
     }
-    const int rg = tid >> 4, cg = tid & 15;  // rows rg * 4 .. + 3; tokens cg, cg + 16; dims cg * 4 and cg * 4 + 64
     float acc[4][8];
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -96,17 +117,25 @@ template <typename T> __global__ void __launch_bounds__(kThreads) tree_simt_kern
             row_s[tid] = row;
         }
         __syncthreads();
-        for (int i = tid; i < kTokens * D4; i += kThreads) {
-            const int t = i / D4, e = i % D4;
-            const int64_t row = row_s[t];
-            float k = 0.f, v = 0.f;
-            if (row >= 0 && e < D) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int e = cg * 4 + h * 64;
+            if (e >= D4) break;
+            float4 k[kTokens / 8], v[kTokens / 8];
+#pragma unroll
+            for (int i = 0; i < kTokens / 8; ++i) {
+                const int64_t row = row_s[rg + 8 * i];
+                k[i] = v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (row < 0) continue;
                 const int64_t at = (row * p.kv_heads + kv_head) * D + e;
-                k = to_float<T>(static_cast<const T *>(p.k)[at]);
-                v = to_float<T>(static_cast<const T *>(p.v)[at]);
+                k[i] = load4<T>(static_cast<const T *>(p.k) + at, p.vectors, D - e);
+                v[i] = load4<T>(static_cast<const T *>(p.v) + at, p.vectors, D - e);
             }
-            k_s[t * stride + e] = k;
-            v_s[t * stride + e] = v;
+#pragma unroll
+            for (int i = 0; i < kTokens / 8; ++i) {
+                *reinterpret_cast<float4 *>(k_s + (rg + 8 * i) * stride + e) = k[i];
+                *reinterpret_cast<float4 *>(v_s + (rg + 8 * i) * stride + e) = v[i];
+            }
         }
         __syncthreads();
         float x[4][2];
@@ -201,46 +230,63 @@ template <typename T> __global__ void __launch_bounds__(kThreads) tree_simt_kern
     }
 }
 
-// Joins the chunks of the rows of one sequence's drafted token: LSE = log sum exp(LSE_i), O = sum exp(LSE_i - LSE) O_i, in chunk order.
+// Joins the chunks of the rows of one sequence's drafted token: LSE = log sum exp(LSE_i), O = sum exp(LSE_i - LSE) O_i, a head a
+// warp.  Lanes take chunks for the weights and dims for the sum, which goes in chunk order.
 template <typename T> __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__ TreeParams p) {
+    __shared__ float w_s[4][kMaxSplits];
     grid_dependency_wait();
     grid_dependency_launch();
-    const int seq = blockIdx.z, node = blockIdx.y;
-    const TreeSequence s = span_of(p, seq);
+    const int seq = blockIdx.z, node = blockIdx.y, lane = threadIdx.x & 31;
+    const TreeSequence s = tree_sequence(p, seq);
     if (node >= s.nodes) return;
     const int parts = max(1, (s.tokens + p.chunk - 1) / p.chunk), D = p.head_dim;
     const int64_t rows = (int64_t)p.max_q * p.q_heads;
-    for (int head = blockIdx.x * 4 + (threadIdx.x >> 5); head < p.q_heads; head += gridDim.x * 4) {
-        const int64_t row = (int64_t)(s.first + node) * p.q_heads + head;
-        float mx = -INFINITY, sum = 0.f;
-        for (int i = 0; i < parts; ++i) mx = fmaxf(mx, p.partial_lse[i * rows + row]);
-        const float base = mx == -INFINITY ? 0.f : mx;
-        for (int i = 0; i < parts; ++i) sum += expf(p.partial_lse[i * rows + row] - base);
-        const bool empty = sum == 0.f;
-        const float total = empty ? -INFINITY : base + logf(sum);
-        for (int d = threadIdx.x & 31; d < D; d += 32) {
-            float o = 0.f;
-            for (int i = 0; i < parts; ++i) {
-                const float w = empty ? 0.f : expf(p.partial_lse[i * rows + row] - total);
-                o = fmaf(w, p.partial_o[(i * rows + row) * D + d], o);
-            }
-            static_cast<T *>(p.o)[row * D + d] = from_float<T>(o);
-        }
-        if ((threadIdx.x & 31) == 0) p.lse[row] = total;
+    float *w = w_s[threadIdx.x >> 5];
+    const int head = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (head >= p.q_heads) return;
+    const int64_t row = (int64_t)(s.first + node) * p.q_heads + head;
+    float mx = -INFINITY, sum = 0.f;
+    for (int i = lane; i < parts; i += 32) {
+        const float x = p.partial_lse[i * rows + row];
+        w[i] = x;
+        mx = x > mx || x != x ? x : mx;
     }
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) {
+        const float x = __shfl_xor_sync(0xffffffffu, mx, d);
+        mx = x > mx || x != x ? x : mx;  // a NaN stays one
+    }
+    const float base = mx == -INFINITY ? 0.f : mx;
+    for (int i = lane; i < parts; i += 32) sum += w[i] = expf(w[i] - base);
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    __syncwarp();
+    const bool empty = sum == 0.f;
+    const float inv = empty ? 0.f : 1.0f / sum;
+    for (int d = lane; d < D; d += 32) {
+        float o = 0.f;
+#pragma unroll 8
+        for (int i = 0; i < parts; ++i) {
+            const float x = p.partial_o[(i * rows + row) * D + d];
+            o = fmaf(w[i], x, o);  // a chunk in which the row sees nothing holds zeros
+        }
+        static_cast<T *>(p.o)[row * D + d] = from_float<T>(o * inv);
+    }
+    if (lane == 0) p.lse[row] = empty ? -INFINITY : base + logf(sum);
 }
 
 template <typename T> int launch(flat_ctx *ctx, TreeParams &p) {
     const int tiles = (int)(((int64_t)p.max_nodes * p.group + kRows - 1) / kRows);
     if ((int64_t)tiles * p.kv_heads > 65535)
         return fail(ctx, FLAT_ERR_DISPATCH_LIMIT, "%d drafted tokens of %d heads are more row tiles than one launch has", p.max_nodes, p.q_heads);
-    // chunks of the longest context that fill the device about four times, 128 tokens at least, as many as the scratch holds
+    // chunks of the longest context that fill the device about four times, a tile of 32 tokens at least, as many as the scratch holds
     const int64_t rows = (int64_t)p.max_q * p.q_heads, units = (int64_t)tiles * p.kv_heads * p.num_seqs;
     const int64_t fit = (int64_t)((kPagedScratchBytes - kPagedPlanBytes) / (rows * (p.head_dim + 1) * sizeof(float)));
-    int64_t splits = std::min<int64_t>({(p.max_context + 127) / 128, std::max<int64_t>(1, (int64_t)ctx->sm_count * 8 / units), 256, fit});
+    int64_t splits = std::min<int64_t>({(p.max_context + kTokens - 1) / kTokens, std::max<int64_t>(1, (int64_t)ctx->sm_count * 4 / units), kMaxSplits, fit});
     if (splits < 1) splits = 1;
     p.chunk = (int)((p.max_context + splits - 1) / splits + kTokens - 1) / kTokens * kTokens;
     p.splits = (int)((p.max_context + p.chunk - 1) / p.chunk);
+    p.vectors = p.head_dim % 4 == 0 && ((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) % (4 * sizeof(T)) == 0;
     p.partial_o = reinterpret_cast<float *>(static_cast<char *>(ctx->paged_scratch) + kPagedPlanBytes);
     p.partial_lse = p.partial_o + p.splits * rows * p.head_dim;
     const int stride = (p.head_dim + 3) / 4 * 4 + 4;
