@@ -1,0 +1,719 @@
+// Attention of few drafted tokens over a paged cache on the tensor cores: at most 64 rows a (sequence, KV head); bf16, head_dim 64 or
+// 128, pages of a multiple of 16 tokens.
+//
+//   rows: (drafted token, head of the group), n * G of them, all against the same keys and values
+//   S = Q K^T (SS MMA, 128 rows x 64 tokens)  ->  P = exp2(S - m)  ->  O += P V (A operand from TMEM)
+//
+// Bound by the bytes of K and V, read once: what counts is that the SM always has tiles on their way.  The beginning and the end of an
+// item (queries read, turned and written; the first scores; the last weights; results) are a chain of 10000 clk and more, and a load
+// takes 2000 clk while K and V stream in.  So nothing of it stands between two tiles:
+//   two CTAs share an SM, 112 KB and half the TMEM each;
+//   K and V tiles of 64 tokens come by TMA, a box per page or tile, through a ring that runs on whatever item is at hand;
+//   one warp plans: it walks the span two items ahead of the products and puts what the other warps have to know in shared memory;
+//   two warps make the next item's queries as soon as the last scores of the item before are formed;
+//   two warps work a softmax row per thread, without shuffles, and write results, while the next item's first scores are formed;
+//   one thread issues all products.  Two score tiles alternate; P lies over the scores it comes from, and the products of one
+//   thread execute in order, so the scores after next cannot overtake the product that reads that P.
+// Half the rows of a product are whatever lies behind the queries in shared memory: a product of 64 rows takes as long.
+//
+// Work: the tiles of all (sequence, KV head) items stand in one line, which is cut into equal spans, one per CTA, whatever
+// the lengths are.  Every CTA adds the lengths up itself, so nothing is planned on the host.  An item that a span's end cuts is
+// joined by a small second kernel from the parts, in order; everything else is written directly.
+//
+// Roundings: q enters as the sum of two bf16 numbers (the tensor core takes one type, and K is bf16; q alone would cost 2^-9 of the
+// scores: 1.7 times the error of the bf16 result, where this way is 1.4 times it), P as bf16, sums and statistics are f32.
+// The running maximum is followed only when it grows by more than 2^8, which keeps the accumulator out of the loop; P then
+// reaches 2^8, sums stay far inside f32.
+//
+// Tokens that a row does not see: its score is replaced by -inf.  P = 0 alone would not do for V that is not finite, so another
+// warp goes over the V tiles that hold drafted tokens or the end of a sequence before they are used: rows behind the end (whatever
+// an earlier owner of the page left) become zero, and so do values of drafted tokens that are not finite; these are then added to
+// the rows that see them at the end, where they were met at all.
+#include "tree_tc.cuh"
+
+namespace flat {
+namespace {
+
+using namespace tree_tc;
+
+constexpr int kTok = 64, kRows = 64, kAhead = 2;  // kAhead: score tiles
+constexpr int kSoftmaxWarps = 2, kQWarp = 2, kQWarps = 2, kKWarp = 4, kVWarp = 5, kMmaWarp = 6;  // ... and one that goes over V tiles
+constexpr int kThreads = 256, kCtasPerSm = 2;
+constexpr int kSegRing = 4;      // see plan
+constexpr int kValidRing = 16;   // tiles between the producer and the slowest softmax warp: the ring's and four more
+constexpr int kPoisonRing = 16;  // segments between the fixing warp and the slowest softmax warp
+
+// A K or V tile lies in shared memory as [8 tokens][64 dims of D][token of the 8][64 dims]: one TMA box of any number of tokens
+// then writes all D dims.  Queries: [summand][64 dims of D][row][64 dims].
+template <int D> struct Cfg {
+    static constexpr int kBoxes = D / 64;
+    static constexpr int kQBox = kRows * 128, kQTile = kQBox * kBoxes;  // one of the two summands of the queries
+    static constexpr int kGroup = 1024 * kBoxes;                        // 8 tokens
+    static constexpr int kKvTile = kTok / 8 * kGroup;
+    static constexpr int kControl = 1024, kSmem = (228 / kCtasPerSm - 1) * 1024;  // of an SM's 228 KB, 1 KB a CTA is the system's
+    static constexpr int kStages = (kSmem - kControl - 2 * kQTile) / kKvTile;     // D = 128: 5, D = 64: 12
+    static_assert(2 * kQTile - kQBox + kMmaRows * 128 <= 2 * kQTile + kStages * kKvTile, "what a product reads behind the queries");
+};
+
+struct Record {  // an item that begins in this CTA and ends in a later one
+    int first, kv_head, rows, parts;
+};
+struct KernelParams {
+    TreeParams t;
+    CUtensorMap map_k, map_v;
+    uint32_t idesc_qk, idesc_pv;
+    int box_rows;      // tokens of a TMA box: 16, 32 or 64, a divisor of the page size
+    float4 *part_o;    // [2 per CTA][D / 4][kRows], not normalised
+    float2 *part_ml;   // [2 per CTA][kRows] maximum (log2 domain) and sum
+    Record *records;   // [CTA]
+};
+
+// A part of an item that one CTA works on.
+struct Segment {
+    TreeSequence s;
+    int seq, kv_head, rows;
+    int j0, n, tiles;  // its first tile, its tiles, the item's
+    int parts;         // of an item that begins here and is cut; otherwise 0
+    int last;          // no segment follows
+};
+
+__device__ __forceinline__ int tiles_of(const TreeSequence &s) { return max(1, (s.tokens + kTok - 1) / kTok); }
+__device__ __forceinline__ int64_t units_of(const TreeParams &p, const TreeSequence &s) {
+    return s.nodes == 0 ? 0 : (int64_t)p.kv_heads * tiles_of(s);
+}
+
+// A CTA's way along its span.
+struct Walk {
+    int64_t at, end, seq_start, units, span;
+    int seq;
+    TreeSequence s;  // of seq
+    __device__ __forceinline__ bool next(const TreeParams &p, Segment &g) {
+        if (at >= end) return false;
+        while (at >= seq_start + units) {
+            seq_start += units;
+            s = tree_sequence(p, ++seq);
+            units = units_of(p, s);
+        }
+        const int tiles = tiles_of(s);
+        const int64_t x = at - seq_start, item = quotient(x, tiles), item_end = seq_start + (item + 1) * tiles;
+        g.s = s;
+        g.seq = seq;
+        g.kv_head = (int)item;
+        g.rows = s.nodes * p.group;
+        g.tiles = tiles;
+        g.j0 = (int)(x - item * tiles);
+        g.n = (int)min((int64_t)(tiles - g.j0), end - at);
+        g.parts = g.j0 == 0 && g.n < tiles ? (int)((item_end - 1) / span) - (int)blockIdx.x + 1 : 0;
+        at += g.n;
+        g.last = at >= end;
+        return true;
+    }
+};
+
+__device__ __forceinline__ void record_timeout(const KernelParams &p, int where) {
+    p.t.status->code = FLAT_ERR_DEVICE_WAIT_TIMEOUT;
+    p.t.status->where = where;
+}
+
+// Whether tile j of the segment's item holds drafted tokens or is its last: its V tile is gone over before it is used.  (Every
+// item has such a tile, so the warp that does it is never more than the ring ahead.)
+__device__ __forceinline__ bool is_tail(const Segment &g, int j) { return (j + 1) * kTok > g.s.len || j + 1 == g.tiles; }
+
+// What the warps of a CTA share, at the start of its shared memory.
+template <int D, int STAGES> struct Control {
+    uint64_t bars[4 * STAGES + 8 + kSegRing];
+    uint64_t turns[D / 2];
+    union {
+        Segment seg[kSegRing];
+        struct {  // before the first is planned
+            int64_t sums[kThreads / 32], totals[kThreads / 32];
+            int64_t seq_start, units;
+            TreeSequence s;
+            int seq;
+        } start;
+    };
+    uint32_t tmem;
+    int abort;
+    uint8_t valid[kValidRing], poison[kPoisonRing];
+};
+
+template <int D> __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __grid_constant__ KernelParams p) {
+    using C = Cfg<D>;
+    using Ctl = Control<D, C::kStages>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    Ctl &ctl = *reinterpret_cast<Ctl *>(smem);
+    static_assert(sizeof(Ctl) <= C::kControl, "control block");
+    uint8_t *q_s = smem + C::kControl;       // [summand]
+    uint8_t *kv_s = q_s + 2 * C::kQTile;     // ring
+    volatile int *abort_flag = &ctl.abort;
+
+    const uint32_t bar0 = smem_u32(ctl.bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };                        // tile landed
+    auto empty = [&](int s) { return bar0 + 8u * (C::kStages + s); };        // tile used
+    auto fixed = [&](int s) { return bar0 + 8u * (2 * C::kStages + s); };    // V tile with drafted tokens gone over
+    auto to_fix = [&](int s) { return bar0 + 8u * (3 * C::kStages + s); };   // such a tile has been requested
+    auto s_full = [&](int b) { return bar0 + 8u * (4 * C::kStages + b); };       // scores in tile b
+    auto p_full = [&](int b) { return bar0 + 8u * (4 * C::kStages + 2 + b); };   // P written over tile b
+    auto pv_done = [&](int b) { return bar0 + 8u * (4 * C::kStages + 4 + b); };  // ... and used
+    const uint32_t q_ready = bar0 + 8u * (4 * C::kStages + 6);                   // queries of the segment written
+    const uint32_t q_empty = bar0 + 8u * (4 * C::kStages + 7);                   // ... and not needed any more
+    auto planned = [&](int k) { return bar0 + 8u * (4 * C::kStages + 8 + k % kSegRing); };  // segment k
+
+    const int warp = warp_index_uniform(), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+            mbar_init(fixed(s), 1);
+            mbar_init(to_fix(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(s_full(b), 1);
+            mbar_init(p_full(b), kSoftmaxWarps);
+            mbar_init(pv_done(b), 1);
+        }
+        mbar_init(q_ready, kQWarps);
+        mbar_init(q_empty, 1);
+        for (int k = 0; k < kSegRing; ++k) mbar_init(planned(k), 1);
+        mbar_fence_init();
+        fence_proxy_async();
+        tma_prefetch_desc(&p.map_k);
+        tma_prefetch_desc(&p.map_v);
+    }
+    if (threadIdx.x < D / 2) ctl.turns[threadIdx.x] = p.t.freq.turns[threadIdx.x];
+    if (warp == kMmaWarp) {
+        tmem_alloc(smem_u32(&ctl.tmem), 512 / kCtasPerSm);
+        tmem_relinquish();
+    }
+    grid_dependency_wait();
+    grid_dependency_launch();
+
+    // The line's length, and the sequence that this CTA's span starts in: a scan over the first kThreads sequences, which mostly are
+    // all there are, with the others' sum beside it.
+    TreeSequence mine{};
+    int64_t units = 0, upto, total = 0;
+    if ((int)threadIdx.x < p.t.num_seqs) {
+        mine = tree_sequence(p.t, threadIdx.x);
+        units = units_of(p.t, mine);
+        if (mine.code && blockIdx.x == 0) tree_report(p.t, mine.code, threadIdx.x);
+    }
+    for (int seq = threadIdx.x + kThreads; seq < p.t.num_seqs; seq += kThreads) {
+        const TreeSequence s = tree_sequence(p.t, seq);
+        total += units_of(p.t, s);
+        if (s.code && blockIdx.x == 0) tree_report(p.t, s.code, seq);
+    }
+    auto scan = [&](int64_t x) {
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += y;
+        }
+        return x;
+    };
+    upto = scan(units);
+    total += units;
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    if (lane == 31) ctl.start.sums[warp] = upto;
+    if (lane == 0) ctl.start.totals[warp] = total;
+    if (threadIdx.x == 0) p.records[blockIdx.x].parts = 0;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    total = 0;
+    int64_t pass = 0;
+    for (int i = 0; i < kThreads / 32; ++i) {
+        if (i < warp) upto += ctl.start.sums[i];
+        pass += ctl.start.sums[i];
+        total += ctl.start.totals[i];
+    }
+    const int64_t span = max((int64_t)1, quotient(total + gridDim.x - 1, (int)gridDim.x));
+    const int64_t begin = min(total, span * blockIdx.x), end = min(total, begin + span);
+    if (begin < end) {
+        int64_t before = 0;  // units of the sequences of earlier passes
+        for (int base = 0;;) {
+            if (begin < upto && begin >= upto - units) {
+                ctl.start.seq = base + threadIdx.x;
+                ctl.start.seq_start = upto - units;
+                ctl.start.units = units;
+                ctl.start.s = mine;
+            }
+            before += pass;
+            if (before > begin) break;
+            base += kThreads;
+            units = 0;
+            if (base + (int)threadIdx.x < p.t.num_seqs) {
+                mine = tree_sequence(p.t, base + threadIdx.x);
+                units = units_of(p.t, mine);
+            }
+            upto = scan(units);
+            __syncthreads();
+            if (lane == 31) ctl.start.sums[warp] = upto;
+            __syncthreads();
+            pass = 0;
+            for (int i = 0; i < kThreads / 32; ++i) {
+                if (i < warp) upto += ctl.start.sums[i];
+                pass += ctl.start.sums[i];
+            }
+            upto += before;
+        }
+    }
+    __syncthreads();
+    const uint32_t tmem_base = ctl.tmem;
+    auto col_s = [](int b) { return (uint32_t)(D + b * kTok); };  // O in columns 0 .. D - 1
+    bool ok = true;
+    auto segment = [&](int k) -> const Segment & {  // waits until it is planned
+        if (!mbar_wait_warp(planned(k), (k / kSegRing) & 1, abort_flag)) {
+            if (lane == 0) record_timeout(p, 500 + warp);
+            ok = false;
+        }
+        return ctl.seg[k % kSegRing];
+    };
+
+    if (begin >= end) {  // nothing to do
+    } else if (warp < kSoftmaxWarps) {
+        // ================= softmax and results =================
+        const uint32_t lanes = (uint32_t)warp << 21;  // this warp's quarter of the TMEM lanes
+        const int row = threadIdx.x;
+        int count = 0;  // tiles so far
+        for (int k = 0;; ++k) {
+            const Segment &g = segment(k);
+            if (!ok) break;
+            const int rows = g.rows, n = g.n, j0 = g.j0, len = g.s.len;
+            const bool live = row < rows, warp_live = warp * 32 < rows;
+            const int node = live ? row / p.t.group : 0;
+            uint32_t own0 = 0, own1 = 0;  // first mask bits
+            if (p.t.mask && live) {
+                const uint32_t *bits = p.t.mask + (int64_t)(g.s.first + node) * p.t.mask_words;
+                own0 = bits[0];
+                if (p.t.mask_words > 1) own1 = bits[1];
+            }
+            float m = -INFINITY, l = 0.f;
+            for (int i = 0; i < n; ++i, ++count) {
+                const int b = count & 1;
+                if (!mbar_wait_warp(s_full(b), (count >> 1) & 1, abort_flag)) {
+                    if (lane == 0) record_timeout(p, 300 + b);
+                    ok = false;
+                    break;
+                }
+                if (warp_live) {
+                    tc_fence_after();
+                    uint32_t x[kTok];
+                    tmem_ld32(tmem_base + lanes + col_s(b), x);
+                    tmem_ld32(tmem_base + lanes + col_s(b) + 32, x + 32);
+                    const uint32_t valid = *reinterpret_cast<volatile uint8_t *>(&ctl.valid[count % kValidRing]);  // 16-token groups whose page is in the pool
+                    const int t0 = (j0 + i) * kTok;
+                    const bool masked = t0 + kTok > len || valid != 0xf;
+                    uint64_t on = ~0ull;
+                    if (masked) {
+                        on = visible(p.t, g.s, node, t0, own0 | (uint64_t)own1 << 32);
+                        for (int e = 0; e < 4; ++e)
+                            if (!((valid >> e) & 1)) on &= ~(0xffffull << (16 * e));
+                    }
+                    tc_wait_ld();
+                    if (masked) {
+                        const uint32_t on0 = (uint32_t)on, on1 = (uint32_t)(on >> 32);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            if (!((on0 >> e) & 1)) x[e] = 0xff800000u;  // -inf
+                            if (!((on1 >> e) & 1)) x[32 + e] = 0xff800000u;
+                        }
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int e = 0; e < kTok; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(x[e]));
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    const bool grows = live && top > m + (i ? kRescaleThreshold : 0.f);
+                    if (__any_sync(0xffffffffu, grows)) {
+                        const float now = grows ? top : m, f = grows ? ex2(m - now) : 1.f;  // m = -inf gives 0
+                        m = now;
+                        l *= f;
+                        if (i > 0) {  // the accumulator, which the value product before this tile still writes
+                            if (!mbar_wait_warp(pv_done(b ^ 1), ((count - 1) >> 1) & 1, abort_flag)) {
+                                if (lane == 0) record_timeout(p, 310 + b);
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 16) {
+                                uint32_t o[16];
+                                tmem_ld16(tmem_base + lanes + c, o);
+                                tc_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                                tmem_st16(tmem_base + lanes + c, o);
+                            }
+                        }
+                    }
+                    const float base = m == -INFINITY ? 0.f : m;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            const float pa = ex2(__uint_as_float(x[32 * h + e]) - base), pb = ex2(__uint_as_float(x[32 * h + e + 1]) - base);
+                            sum[(e >> 1) & 3] += pa + pb;
+                            x[32 * h + e / 2] = pack_bf16(pa, pb);
+                        }
+                        tmem_st16(tmem_base + lanes + col_s(b) + 16 * h, x + 32 * h);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tc_wait_st();
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(b));
+            }
+            if (!ok) break;
+            // ---- results, while the next segment's first scores are formed
+            if (!mbar_wait_warp(pv_done((count - 1) & 1), ((count - 1) >> 1) & 1, abort_flag)) {
+                if (lane == 0) record_timeout(p, 320);
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            if (warp_live) {
+                const bool whole = n == g.tiles, nothing = l == 0.f;
+                const int64_t part = (int64_t)blockIdx.x * 2 + (j0 == 0 ? 1 : 0);
+                const int64_t out = (int64_t)(g.s.first + node) * p.t.q_heads + g.kv_head * p.t.group + (live ? row - node * p.t.group : 0);
+                const float keep = nothing ? 0.f : whole ? 1.0f / l : 1.f;
+                const int poison = *reinterpret_cast<volatile uint8_t *>(&ctl.poison[k % kPoisonRing]);
+                if (live) {
+                    if (whole) p.t.lse[out] = nothing ? -INFINITY : (m + log2f(l)) * kLn2;
+                    else p.part_ml[part * kRows + row] = make_float2(m, l);
+                }
+                uint4 *to = reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.t.o) + out * D);
+                float4 *to_part = p.part_o + part * (D / 4) * kRows + row;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 16) {
+                    uint32_t raw[16];
+                    float o[16];
+                    tmem_ld16(tmem_base + lanes + c, raw);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] = nothing ? 0.f : __uint_as_float(raw[e]) * keep;
+                    if (!live) continue;
+                    if (poison) add_not_finite(p.t, g.s, g.seq, g.kv_head, node, j0 * kTok, (j0 + n) * kTok, c, o);
+                    if (whole) {
+                        to[c / 8] = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
+                        to[c / 8 + 1] = make_uint4(pack_bf16(o[8], o[9]), pack_bf16(o[10], o[11]), pack_bf16(o[12], o[13]), pack_bf16(o[14], o[15]));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) to_part[(c / 4 + e) * kRows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    }
+                }
+            }
+            tc_fence_before();  // the next segment's first value product starts the accumulator anew, behind this warp's next P
+            if (threadIdx.x == 0 && g.parts) p.records[blockIdx.x] = Record{g.s.first, g.kv_head, rows, g.parts};
+            if (g.last) break;
+        }
+    } else if (warp < kQWarp + kQWarps) {
+        // ================= planning; queries =================
+        // A segment is planned once the queries of the one two before it are not needed any more.  By then its last scores have been
+        // asked for, and with them the value products of the segment before: no warp has to do with anything before that one, which is three
+        // before the planned one, and the ring holds four.
+        const bool plans = warp == kQWarp;
+        Walk walk{};
+        Segment coming;
+        bool more = false;
+        auto publish = [&](int k) {
+            if (lane == 0) {
+                ctl.seg[k % kSegRing] = coming;
+                mbar_arrive(planned(k));
+            }
+            __syncwarp();
+        };
+        if (plans) {
+            walk = Walk{begin, end, ctl.start.seq_start, ctl.start.units, span, ctl.start.seq, ctl.start.s};
+            __syncwarp();
+            walk.next(p.t, coming);
+            publish(0);
+            more = walk.next(p.t, coming);
+            if (more) publish(1);
+        }
+        const int tid = threadIdx.x - kQWarp * 32, quads = (p.t.group + 3) / 4;
+        for (int k = 0;; ++k) {
+            const Segment &g = segment(k);
+            if (!ok) break;
+            const int last = g.last, tasks = g.s.nodes * quads * (D / 8), head0 = g.kv_head * p.t.group, first = g.s.first;
+            // A thread takes 8 dims of up to four heads of a drafted token, whose angles are the same.  The loads of a step are
+            // all in flight during the step before; the first ones while the last scores of the segment before are formed.
+            struct Raw {
+                uint4 q[4];
+                int position;
+            } now, next;
+            auto request = [&](int i, Raw &x) {
+                const int c = i % (D / 8), nq = i / (D / 8), node = nq / quads, h = nq % quads * 4;
+                x.position = p.t.positions[first + node];
+                const char *from = static_cast<const char *>(p.t.q) + (((int64_t)(first + node) * p.t.q_heads + head0 + h) * D + c * 8) * 2;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (h + e < p.t.group) x.q[e] = *reinterpret_cast<const uint4 *>(from + e * D * 2);
+            };
+            if (tid < tasks) request(tid, now);
+            for (int i = tid; i < g.rows * C::kBoxes; i += kQWarps * 32) {  // the later steps', 128 bytes each
+                const int r = i / C::kBoxes, node = r / p.t.group;
+                const char *at = static_cast<const char *>(p.t.q) + ((int64_t)(first + node) * p.t.q_heads + head0 + r - node * p.t.group) * (D * 2) + i % C::kBoxes * 128;
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+            }
+            if (k > 0) {
+                if (plans && more) more = walk.next(p.t, coming);
+                if (!mbar_wait_warp(q_empty, (k - 1) & 1, abort_flag)) {
+                    if (lane == 0) record_timeout(p, 330);
+                    ok = false;
+                    break;
+                }
+                if (plans && more) publish(k + 1);
+            }
+#pragma unroll 1
+            for (int i = tid; i < tasks; i += kQWarps * 32) {
+                if (i + kQWarps * 32 < tasks) request(i + kQWarps * 32, next);
+                const int c = i % (D / 8), nq = i / (D / 8), node = nq / quads, h = nq % quads * 4;
+                float2 cs[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    cs[e] = turn_of_fast(now.position, ctl.turns[c * 4 + e]);
+                    cs[e].x *= p.t.scale * kLog2e;
+                    cs[e].y *= p.t.scale * kLog2e;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = node * p.t.group + h + e;
+                    if (h + e < p.t.group) write_query<C::kQTile>(now.q[e], cs, q_s + (c >> 3) * C::kQBox + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                }
+                now = next;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_ready);
+            if (last) break;
+        }
+    } else if (warp == kKWarp || warp == kVWarp) {
+        // ================= TMA producers: K tiles and V tiles =================
+        const bool is_k = warp == kKWarp;
+        const CUtensorMap *map = is_k ? &p.map_k : &p.map_v;
+        const int boxes = kTok / p.box_rows, groups = p.box_rows / 8, page_groups = p.t.page_size / 8;
+        const int no_group = p.t.physical_pages * page_groups;  // behind the pool: zeros
+        uint32_t order = 0;  // tiles of the ring before the segment
+        int count = 0;
+        for (int k = 0;; ++k) {
+            const Segment g = segment(k);
+            if (!ok) break;
+            BoxRows rows;
+            rows.start(p.t, g.seq, g.s.tokens, g.j0 * kTok, p.box_rows);
+            for (int i = 0; i < g.n; ++i, ++count) {
+                const int first = (g.j0 + i) * boxes;
+                rows.seek(first);
+                const bool bad = rows.page == -1 || rows.page >= p.t.physical_pages;
+                const int group = rows.page < 0 || bad ? no_group : rows.page * page_groups + (rows.in_page >> 3);
+                if (is_k) {
+                    uint32_t valid = 0xf;
+                    const uint32_t all = __ballot_sync(0xffffffffu, bad) >> (first - rows.base);
+                    if (all) {
+                        for (int e = 0; e < 4; ++e)
+                            if ((all >> (e * 16 / p.box_rows)) & 1 && e * 16 / p.box_rows < boxes) valid &= ~(1u << e);
+                        if (lane == 0 && valid != 0xf) tree_report(p.t, FLAT_ERR_PAGE_OUT_OF_RANGE, g.seq);
+                    }
+                    if (lane == 0) ctl.valid[count % kValidRing] = (uint8_t)valid;
+                }
+                const uint32_t at = order + (is_k ? k_entry(i, kAhead) : v_entry(i, g.n, kAhead));
+                const int s = at % C::kStages;
+                if (!mbar_wait_warp(empty(s), ((at / C::kStages) & 1) ^ 1, abort_flag)) {
+                    if (lane == 0) record_timeout(p, 100 + s);
+                    ok = false;
+                    break;
+                }
+                __syncwarp();
+                const bool leader = elect_one();
+                if (leader) mbar_expect_tx(full(s), C::kKvTile);
+                const uint32_t dst = smem_u32(kv_s + s * C::kKvTile);
+                for (int b = 0; b < boxes; ++b) {
+                    const int from = __shfl_sync(0xffffffffu, group, first - rows.base + b);
+                    if (leader) tma_load_5d(dst + b * groups * C::kGroup, map, from, g.kv_head, full(s));
+                }
+                if (!is_k && leader && is_tail(g, g.j0 + i)) mbar_arrive(to_fix(s));
+            }
+            if (!ok || g.last) break;
+            order += 2 * g.n;
+        }
+    } else if (warp == kMmaWarp) {
+        // ================= all products =================
+        if (elect_one()) {
+            const uint32_t q_desc = (uint32_t)make_smem_desc(smem_u32(q_s), 0, 1024);
+            const uint32_t k_desc = (uint32_t)make_smem_desc(smem_u32(kv_s), 0, C::kGroup);
+            const uint32_t v_desc = (uint32_t)make_smem_desc(smem_u32(kv_s), 1024, C::kGroup);
+            constexpr uint32_t kTile16 = C::kKvTile >> 4;
+            uint32_t order = 0, fixed_phase = 0;
+            int done = 0;  // tiles of the segments before
+            auto wait = [&](uint32_t bar, uint32_t parity, int where) {
+                if (ok && !mbar_wait(bar, parity, abort_flag)) {
+                    record_timeout(p, where);
+                    ok = false;
+                }
+            };
+            auto landed = [&](int entry) {  // waits for a tile of the segment; its stage
+                const uint32_t at = order + entry;
+                wait(full(at % C::kStages), (at / C::kStages) & 1, 210);
+                return (int)(at % C::kStages);
+            };
+            auto scores = [&](int i, int n) {
+                const int b = (done + i) & 1, s = landed(k_entry(i, kAhead));
+                if (!ok) return;
+                tc_fence_after();
+                const uint32_t kk = k_desc + s * kTile16, d = tmem_base + col_s(b);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)  // the two summands of q
+#pragma unroll
+                    for (int e = 0; e < D / 16; ++e)
+                        mma_scores<C::kGroup>(d, q_desc + h * (C::kQTile >> 4) + (e >> 2) * (C::kQBox >> 4) + (e & 3) * 2,
+                                              kk + (e >> 2) * (1024 >> 4) + (e & 3) * 2, p.idesc_qk, h > 0 || e > 0);
+                tc_commit(s_full(b));
+                tc_commit(empty(s));
+                if (i + 1 == n) tc_commit(q_empty);
+            };
+            for (int k = 0;; ++k) {
+                wait(planned(k), (k / kSegRing) & 1, 506);
+                wait(q_ready, k & 1, 200);
+                if (!ok) break;
+                const Segment g = ctl.seg[k % kSegRing];
+                for (int i = 0; i < min(g.n, kAhead); ++i) scores(i, g.n);
+                for (int v = 0; ok && v < g.n; ++v) {
+                    const int b = (done + v) & 1, s = landed(v_entry(v, g.n, kAhead));
+                    if (is_tail(g, g.j0 + v)) {
+                        wait(fixed(s), (fixed_phase >> s) & 1, 230);
+                        fixed_phase ^= 1u << s;
+                    }
+                    wait(p_full(b), ((done + v) >> 1) & 1, 240 + b);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int e = 0; e < kTok / 16; ++e)
+                        mma_values<C::kGroup>(tmem_base, tmem_base + col_s(b) + e * 8, v_desc + s * kTile16 + e * (2 * C::kGroup >> 4), p.idesc_pv,
+                                              v > 0 || e > 0);
+                    tc_commit(pv_done(b));
+                    tc_commit(empty(s));
+                    if (v + kAhead < g.n) scores(v + kAhead, g.n);
+                }
+                if (!ok || g.last) break;
+                done += g.n;
+                order += 2 * g.n;
+            }
+        }
+    } else {
+        // ================= V tiles with drafted tokens or the end of a sequence =================
+        uint32_t order = 0, phase = 0;
+        for (int k = 0;; ++k) {
+            const Segment g = segment(k);
+            if (!ok) break;
+            if (lane == 0) ctl.poison[k % kPoisonRing] = 0;
+            __syncwarp();
+            // (to_fix tells that the tile before in this stage is used up, without which its phase could be taken for this one's)
+            for (int v = max(0, min(g.s.len / kTok, g.tiles - 1) - g.j0); v < g.n; ++v) {
+                const uint32_t at = order + v_entry(v, g.n, kAhead);
+                const int s = at % C::kStages;
+                if (!mbar_wait_warp(to_fix(s), (phase >> s) & 1, abort_flag) || !mbar_wait_warp(full(s), (at / C::kStages) & 1, abort_flag)) {
+                    if (lane == 0) record_timeout(p, 400);
+                    ok = false;
+                    break;
+                }
+                phase ^= 1u << s;
+                const int t0 = (g.j0 + v) * kTok;
+                const bool met = clear_values<C::kBoxes, kTok>(kv_s + s * C::kKvTile, max(0, min(g.s.len, g.s.tokens) - t0), g.s.tokens - t0);
+                if (__any_sync(0xffffffffu, met) && lane == 0) ctl.poison[k % kPoisonRing] = 1;
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(fixed(s));
+            }
+            if (!ok || g.last) break;
+            order += 2 * g.n;
+        }
+    }
+
+    if (*abort_flag) {
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);  // let copies in flight land before the CTA exits
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512 / kCtasPerSm);
+    }
+}
+
+// Joins the parts of an item that begins in CTA blockIdx.x and ends in a later one, in CTA order: 32 rows a block, a row a lane, D / 8
+// dims a warp.
+template <int D> __global__ void __launch_bounds__(256) tree_few_merge_kernel(const __grid_constant__ KernelParams p) {
+    grid_dependency_wait();
+    grid_dependency_launch();
+    const Record rec = p.records[blockIdx.x];
+    const int warp = threadIdx.x >> 5, r = blockIdx.y * 32 + (threadIdx.x & 31);
+    if (rec.parts <= 0 || r >= rec.rows) return;
+    constexpr int kPer = D / 32;  // groups of four dims
+    auto part = [&](int i) { return (int64_t)((blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)); };
+    float mx = -INFINITY;
+#pragma unroll 4
+    for (int i = 0; i < rec.parts; ++i) mx = fmaxf(mx, p.part_ml[part(i) * kRows + r].x);
+    float sum = 0.f;
+    float4 o[kPer] = {};
+#pragma unroll 2
+    for (int i = 0; i < rec.parts; ++i) {
+        const float2 ml = p.part_ml[part(i) * kRows + r];
+        float4 x[kPer];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) x[e] = p.part_o[(part(i) * (D / 4) + warp * kPer + e) * kRows + r];
+        if (ml.y == 0.f) continue;  // a part in which the row has seen nothing; a NaN counts
+        const float f = ex2(ml.x - mx);
+        sum = fmaf(f, ml.y, sum);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+            o[e] = make_float4(fmaf(f, x[e].x, o[e].x), fmaf(f, x[e].y, o[e].y), fmaf(f, x[e].z, o[e].z), fmaf(f, x[e].w, o[e].w));
+    }
+    const bool nothing = sum == 0.f;
+    const float inv = nothing ? 0.f : 1.0f / sum;
+    const int64_t out = (int64_t)(rec.first + r / p.t.group) * p.t.q_heads + rec.kv_head * p.t.group + r % p.t.group;
+    uint2 *to = reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p.t.o) + out * D + warp * (D / 8));
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) to[e] = make_uint2(pack_bf16(o[e].x * inv, o[e].y * inv), pack_bf16(o[e].z * inv, o[e].w * inv));
+    if (warp == 0) p.t.lse[out] = nothing ? -INFINITY : (mx + log2f(sum)) * kLn2;
+}
+
+template <int D> int launch(flat_ctx *ctx, const TreeParams &t) {
+    using C = Cfg<D>;
+    KernelParams p{};
+    p.t = t;
+    p.box_rows = t.page_size % 64 == 0 ? 64 : t.page_size % 32 == 0 ? 32 : 16;
+    const uint64_t rows = (uint64_t)t.physical_pages * t.page_size;
+    if (int st = make_pool_map(ctx, &p.map_k, t.k, D, rows, t.kv_heads, p.box_rows)) return st;
+    if (int st = make_pool_map(ctx, &p.map_v, t.v, D, rows, t.kv_heads, p.box_rows)) return st;
+    p.idesc_qk = make_idesc(kFmtBF16, kFmtBF16, 0, 0, kMmaRows, kTok);
+    p.idesc_pv = make_idesc(kFmtBF16, kFmtBF16, 0, 1, kMmaRows, D);
+    const int grid = ctx->sm_count * kCtasPerSm;
+    char *at = static_cast<char *>(ctx->paged_scratch) + kPagedPlanBytes;
+    const uint64_t rows_held = (uint64_t)grid * 2 * kRows;
+    const uint64_t o_bytes = rows_held * D * sizeof(float), ml_bytes = rows_held * sizeof(float2);
+    if (o_bytes + ml_bytes + grid * sizeof(Record) > kPagedScratchBytes - kPagedPlanBytes)
+        return fail(ctx, FLAT_ERR_EXECUTION, "the scratch does not hold the parts of %d CTAs", grid);
+    p.part_o = reinterpret_cast<float4 *>(at);
+    p.part_ml = reinterpret_cast<float2 *>(at + o_bytes);
+    p.records = reinterpret_cast<Record *>(at + o_bytes + ml_bytes);
+    FLAT_CUDA_OK(ctx, cudaFuncSetAttribute(tree_few_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    {
+        KernelTimer timer(ctx);
+        FLAT_CUDA_OK(ctx, launch_dependent(may_overlap_previous(ctx), tree_few_kernel<D>, dim3((unsigned)grid), kThreads, C::kSmem, ctx->stream, p));
+    }
+    ctx->launches += 1;
+    const int chunks = (int)(((int64_t)t.max_nodes * t.group + 31) / 32);
+    FLAT_CUDA_OK(ctx, launch_dependent(true, tree_few_merge_kernel<D>, dim3((unsigned)grid, (unsigned)chunks), 256, 0, ctx->stream, p));
+    ctx->launches += 1;
+    return FLAT_OK;
+}
+
+}  // namespace
+
+bool tree_few_supported(const TreeParams &p) { return (int64_t)p.max_nodes * p.group <= kRows; }
+
+int launch_tree_few(flat_ctx *ctx, const TreeParams &p) { return p.head_dim == 128 ? launch<128>(ctx, p) : launch<64>(ctx, p); }
+
+}  // namespace flat
