@@ -784,6 +784,8 @@ int32_t flat_ctx_device_status(flat_ctx *ctx) {
             fail(ctx, h.code, "lengths of sequence %d do not fit its pages or the call's bounds; it was left out", h.where);
         else
             fail(ctx, h.code, "device wait expired at site %d", h.where);
+        if (h.code == FLAT_ERR_DEVICE_WAIT_TIMEOUT && ctx->paged_scratch)  // a kernel that gave up has not counted to the end
+            cudaMemset(paged_tickets(ctx), 0, (kPagedTickets + 1) * sizeof(unsigned));
         cudaMemset(ctx->dev_status, 0, sizeof(DeviceStatus));
     }
     return h.code;
@@ -1849,8 +1851,8 @@ PagedBatchParams batch_params(flat_ctx *ctx, const flat_paged_batch *b) {
     p.plan = static_cast<int4 *>(ctx->paged_scratch);
     p.plan_offsets = reinterpret_cast<int32_t *>(p.plan + kMaxBatchSeqs + 1);
     p.plan_free_count = p.plan_offsets + kMaxBatchSeqs + 1;
-    p.plan_ticket = reinterpret_cast<unsigned *>(p.plan_free_count + 1);
-    static_assert((kMaxBatchSeqs + 1) * (sizeof(int4) + sizeof(int32_t)) + 2 * sizeof(int32_t) <= kPagedPlanBytes, "plan region");
+    p.plan_ticket = paged_tickets(ctx);
+    static_assert((kMaxBatchSeqs + 1) * (sizeof(int4) + sizeof(int32_t)) + (kPagedTickets + 2) * sizeof(int32_t) <= kPagedPlanBytes, "plan region");
     return p;
 }
 

@@ -313,6 +313,10 @@ int launch_append_rows(flat_ctx *ctx, int dtype, const void *k_src, const void *
 constexpr uint64_t kPagedScratchBytes = 48ull << 20;
 constexpr uint64_t kPagedPlanBytes = 2ull << 20;  // plans of reserve and release, at its start: 20 bytes a sequence
 constexpr uint64_t kMaxBatchSeqs = 65535;
+constexpr uint64_t kPagedTickets = 1024;  // counters at the end of the plan region, 0 between calls: one of reserve and release, those of the attention
+inline unsigned *paged_tickets(flat_ctx *ctx) {
+    return reinterpret_cast<unsigned *>(static_cast<char *>(ctx->paged_scratch) + kPagedPlanBytes) - (kPagedTickets + 1);
+}
 int ensure_paged_scratch(flat_ctx *ctx);
 struct PagedBatchParams {
     int num_seqs, page_size, physical_pages, max_pages;

@@ -18,7 +18,7 @@
 //
 // Work: the tiles of all (sequence, KV head) items stand in one line, which is cut into equal spans, one per CTA, whatever
 // the lengths are.  Every CTA adds the lengths up itself, so nothing is planned on the host.  An item that a span's end cuts is
-// joined by a small second kernel from the parts, in order; everything else is written directly.
+// joined, from the parts in order, by the CTA that finds that they are all there; everything else is written directly.
 //
 // Roundings: q enters as the sum of two bf16 numbers (the tensor core takes one type, and K is bf16; q alone would cost 2^-9 of the
 // scores: 1.7 times the error of the bf16 result, where this way is 1.4 times it), P as bf16, sums and statistics are f32.
@@ -39,7 +39,8 @@ using namespace tree_tc;
 constexpr int kTok = 64, kRows = 64, kAhead = 2;  // kAhead: score tiles
 constexpr int kSoftmaxWarps = 2, kQWarp = 2, kQWarps = 2, kKWarp = 4, kVWarp = 5, kMmaWarp = 6;  // ... and one that goes over V tiles
 constexpr int kThreads = 256, kCtasPerSm = 2;
-constexpr int kSegRing = 4;      // see plan
+constexpr int kSegRing = 4;      // see below, planning
+constexpr int kQSteps = 4;       // tokens of a thread of the query warps in flight
 constexpr int kValidRing = 16;   // tiles between the producer and the slowest softmax warp: the ring's and four more
 constexpr int kPoisonRing = 16;  // segments between the fixing warp and the slowest softmax warp
 
@@ -55,9 +56,6 @@ template <int D> struct Cfg {
     static_assert(2 * kQTile - kQBox + kMmaRows * 128 <= 2 * kQTile + kStages * kKvTile, "what a product reads behind the queries");
 };
 
-struct Record {  // an item that begins in this CTA and ends in a later one
-    int first, kv_head, rows, parts;
-};
 struct KernelParams {
     TreeParams t;
     CUtensorMap map_k, map_v;
@@ -65,7 +63,7 @@ struct KernelParams {
     int box_rows;      // tokens of a TMA box: 16, 32 or 64, a divisor of the page size
     float4 *part_o;    // [2 per CTA][D / 4][kRows], not normalised
     float2 *part_ml;   // [2 per CTA][kRows] maximum (log2 domain) and sum
-    Record *records;   // [CTA]
+    unsigned *arrived; // [CTA]: warps that have written their part of the item that begins in this CTA and ends in a later one; 0 between calls
 };
 
 // A part of an item that one CTA works on.
@@ -73,19 +71,16 @@ struct Segment {
     TreeSequence s;
     int seq, kv_head, rows;
     int j0, n, tiles;  // its first tile, its tiles, the item's
-    int parts;         // of an item that begins here and is cut; otherwise 0
+    int parts, cta;    // of an item that is cut, and the CTA that it begins in; otherwise parts = 1
     int last;          // no segment follows
 };
 
 __device__ __forceinline__ int tiles_of(const TreeSequence &s) { return max(1, (s.tokens + kTok - 1) / kTok); }
-__device__ __forceinline__ int64_t units_of(const TreeParams &p, const TreeSequence &s) {
-    return s.nodes == 0 ? 0 : (int64_t)p.kv_heads * tiles_of(s);
-}
+__device__ __forceinline__ int units_of(const TreeParams &p, const TreeSequence &s) { return s.nodes == 0 ? 0 : p.kv_heads * tiles_of(s); }
 
 // A CTA's way along its span.
 struct Walk {
-    int64_t at, end, seq_start, units, span;
-    int seq;
+    int at, end, seq_start, units, span, seq;
     TreeSequence s;  // of seq
     __device__ __forceinline__ bool next(const TreeParams &p, Segment &g) {
         if (at >= end) return false;
@@ -95,15 +90,20 @@ struct Walk {
             units = units_of(p, s);
         }
         const int tiles = tiles_of(s);
-        const int64_t x = at - seq_start, item = quotient(x, tiles), item_end = seq_start + (item + 1) * tiles;
+        const int x = at - seq_start, item = (int)((unsigned)x / (unsigned)tiles), item_start = seq_start + item * tiles;
         g.s = s;
         g.seq = seq;
-        g.kv_head = (int)item;
+        g.kv_head = item;
         g.rows = s.nodes * p.group;
         g.tiles = tiles;
-        g.j0 = (int)(x - item * tiles);
-        g.n = (int)min((int64_t)(tiles - g.j0), end - at);
-        g.parts = g.j0 == 0 && g.n < tiles ? (int)((item_end - 1) / span) - (int)blockIdx.x + 1 : 0;
+        g.j0 = at - item_start;
+        g.n = min(tiles - g.j0, end - at);
+        g.parts = 1;
+        g.cta = blockIdx.x;
+        if (g.n < tiles) {
+            g.cta = (int)((unsigned)item_start / (unsigned)span);
+            g.parts = (int)((unsigned)(item_start + tiles - 1) / (unsigned)span) - g.cta + 1;
+        }
         at += g.n;
         g.last = at >= end;
         return true;
@@ -119,27 +119,79 @@ __device__ __forceinline__ void record_timeout(const KernelParams &p, int where)
 // item has such a tile, so the warp that does it is never more than the ring ahead.)
 __device__ __forceinline__ bool is_tail(const Segment &g, int j) { return (j + 1) * kTok > g.s.len || j + 1 == g.tiles; }
 
+struct Join {  // an item whose parts are all there
+    int first, kv_head, rows, parts, cta;
+};
+
 // What the warps of a CTA share, at the start of its shared memory.
-template <int D, int STAGES> struct Control {
-    uint64_t bars[4 * STAGES + 8 + kSegRing];
-    uint64_t turns[D / 2];
+template <int STAGES> struct Control {
+    uint64_t bars[4 * STAGES + 9 + kSegRing];
     union {
         Segment seg[kSegRing];
         struct {  // before the first is planned
-            int64_t sums[kThreads / 32], totals[kThreads / 32];
-            int64_t seq_start, units;
+            int sums[kThreads / 32];
+            int seq_start, units, seq;
             TreeSequence s;
-            int seq;
         } start;
     };
     uint32_t tmem;
     int abort;
+    Walk walk;     // of the planning warp
+    Segment coming;
+    Join join[2];  // an item that ends here, and one that does not
     uint8_t valid[kValidRing], poison[kPoisonRing];
 };
 
+// Joins the parts of an item in CTA order, whichever came last: a row a thread and a share of the dims; ml_s: every part's statistics.
+template <int D> __device__ __forceinline__ void join_parts(const KernelParams &p, const Join &item, float2 *ml_s) {
+    const int lanes = item.rows <= 32 ? 32 : 64, r = threadIdx.x & (lanes - 1), g = threadIdx.x / lanes, groups = kThreads / lanes, parts = item.parts;
+    const bool live = r < item.rows;
+    const int part0 = item.cta * 2;  // of the first CTA the second part, of the others the first
+    for (int i = g; i < parts; i += groups)
+        if (live) ml_s[i * kRows + r] = __ldcg(&p.part_ml[(int64_t)(part0 + (i == 0 ? 1 : 2 * i)) * kRows + r]);
+    __syncthreads();
+    if (!live) return;
+    float mx = -INFINITY, sum = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < parts; ++i) mx = fmaxf(mx, ml_s[i * kRows + r].x);
+    auto weight = [&](float2 ml) { return ml.y == 0.f ? 0.f : ex2(ml.x - mx); };  // a part in which the row has seen nothing; a NaN counts
+#pragma unroll 1
+    for (int i = 0; i < parts; ++i) sum = fmaf(weight(ml_s[i * kRows + r]), ml_s[i * kRows + r].y, sum);
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const int node = r / p.t.group;
+    const int64_t out = (int64_t)(item.first + node) * p.t.q_heads + item.kv_head * p.t.group + r - node * p.t.group;
+    if (g == 0) p.t.lse[out] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+#pragma unroll 1
+    for (int d4 = g * 4; d4 < D / 4; d4 += groups * 4) {
+        float4 o[4] = {};
+#pragma unroll 1
+        for (int base = 0; base < parts; base += 4) {
+            float4 x[4][4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (base + u < parts) {
+                    const float4 *from = p.part_o + ((int64_t)(part0 + (base + u == 0 ? 1 : 2 * (base + u))) * (D / 4) + d4) * kRows + r;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[u][e] = __ldcg(from + e * kRows);
+                }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (base + u < parts) {
+                    const float f = weight(ml_s[(base + u) * kRows + r]) * inv;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        o[e] = make_float4(fmaf(f, x[u][e].x, o[e].x), fmaf(f, x[u][e].y, o[e].y), fmaf(f, x[u][e].z, o[e].z), fmaf(f, x[u][e].w, o[e].w));
+                }
+        }
+        uint4 *to = reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.t.o) + out * D + d4 * 4);
+        to[0] = make_uint4(pack_bf16(o[0].x, o[0].y), pack_bf16(o[0].z, o[0].w), pack_bf16(o[1].x, o[1].y), pack_bf16(o[1].z, o[1].w));
+        to[1] = make_uint4(pack_bf16(o[2].x, o[2].y), pack_bf16(o[2].z, o[2].w), pack_bf16(o[3].x, o[3].y), pack_bf16(o[3].z, o[3].w));
+    }
+}
+
 template <int D> __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_few_kernel(const __grid_constant__ KernelParams p) {
     using C = Cfg<D>;
-    using Ctl = Control<D, C::kStages>;
+    using Ctl = Control<C::kStages>;
     extern __shared__ __align__(1024) uint8_t smem[];
     Ctl &ctl = *reinterpret_cast<Ctl *>(smem);
     static_assert(sizeof(Ctl) <= C::kControl, "control block");
@@ -157,11 +209,13 @@ template <int D> __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_fe
     auto pv_done = [&](int b) { return bar0 + 8u * (4 * C::kStages + 4 + b); };  // ... and used
     const uint32_t q_ready = bar0 + 8u * (4 * C::kStages + 6);                   // queries of the segment written
     const uint32_t q_empty = bar0 + 8u * (4 * C::kStages + 7);                   // ... and not needed any more
-    auto planned = [&](int k) { return bar0 + 8u * (4 * C::kStages + 8 + k % kSegRing); };  // segment k
+    const uint32_t go = bar0 + 8u * (4 * C::kStages + 8);                        // K and V may be asked for
+    auto planned = [&](int k) { return bar0 + 8u * (4 * C::kStages + 9 + k % kSegRing); };  // segment k
 
     const int warp = warp_index_uniform(), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         *abort_flag = 0;
+        ctl.join[0].parts = ctl.join[1].parts = 0;
         for (int s = 0; s < C::kStages; ++s) {
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
@@ -175,13 +229,13 @@ template <int D> __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_fe
         }
         mbar_init(q_ready, kQWarps);
         mbar_init(q_empty, 1);
+        mbar_init(go, kQWarps);
         for (int k = 0; k < kSegRing; ++k) mbar_init(planned(k), 1);
         mbar_fence_init();
         fence_proxy_async();
         tma_prefetch_desc(&p.map_k);
         tma_prefetch_desc(&p.map_v);
     }
-    if (threadIdx.x < D / 2) ctl.turns[threadIdx.x] = p.t.freq.turns[threadIdx.x];
     if (warp == kMmaWarp) {
         tmem_alloc(smem_u32(&ctl.tmem), 512 / kCtasPerSm);
         tmem_relinquish();
@@ -189,74 +243,57 @@ template <int D> __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_fe
     grid_dependency_wait();
     grid_dependency_launch();
 
-    // The line's length, and the sequence that this CTA's span starts in: a scan over the first kThreads sequences, which mostly are
-    // all there are, with the others' sum beside it.
-    TreeSequence mine{};
-    int64_t units = 0, upto, total = 0;
-    if ((int)threadIdx.x < p.t.num_seqs) {
-        mine = tree_sequence(p.t, threadIdx.x);
-        units = units_of(p.t, mine);
-        if (mine.code && blockIdx.x == 0) tree_report(p.t, mine.code, threadIdx.x);
-    }
-    for (int seq = threadIdx.x + kThreads; seq < p.t.num_seqs; seq += kThreads) {
-        const TreeSequence s = tree_sequence(p.t, seq);
-        total += units_of(p.t, s);
-        if (s.code && blockIdx.x == 0) tree_report(p.t, s.code, seq);
-    }
-    auto scan = [&](int64_t x) {
+    // The line's length, then the sequence that this CTA's span starts in: a scan over kThreads sequences at a time, the same once more
+    // where there are more.  (What runs once is kept short here and below: instructions that are not in the cache yet come at a
+    // tenth of the rate.)
+    int span = 1, begin = 0, end = 0;
+    {
+        int total = 0, before = 0;
+        bool counting = true;
+#pragma unroll 1
+        for (int base = 0;; base += kThreads) {
+            TreeSequence mine{};
+            int units = 0;
+            if (base + (int)threadIdx.x < p.t.num_seqs) {
+                mine = tree_sequence(p.t, base + threadIdx.x);
+                units = units_of(p.t, mine);
+                if (mine.code && counting && blockIdx.x == 0) tree_report(p.t, mine.code, base + threadIdx.x);
+            }
+            int upto = units;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
-            if (lane >= d) x += y;
-        }
-        return x;
-    };
-    upto = scan(units);
-    total += units;
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-    if (lane == 31) ctl.start.sums[warp] = upto;
-    if (lane == 0) ctl.start.totals[warp] = total;
-    if (threadIdx.x == 0) p.records[blockIdx.x].parts = 0;
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    total = 0;
-    int64_t pass = 0;
-    for (int i = 0; i < kThreads / 32; ++i) {
-        if (i < warp) upto += ctl.start.sums[i];
-        pass += ctl.start.sums[i];
-        total += ctl.start.totals[i];
-    }
-    const int64_t span = max((int64_t)1, quotient(total + gridDim.x - 1, (int)gridDim.x));
-    const int64_t begin = min(total, span * blockIdx.x), end = min(total, begin + span);
-    if (begin < end) {
-        int64_t before = 0;  // units of the sequences of earlier passes
-        for (int base = 0;;) {
-            if (begin < upto && begin >= upto - units) {
+            for (int d = 1; d < 32; d <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += y;
+            }
+            if (lane == 31) ctl.start.sums[warp] = upto;
+            tc_fence_before();
+            __syncthreads();
+            tc_fence_after();
+            const int sums = lane < kThreads / 32 ? ctl.start.sums[lane] : 0;
+            const int pass = (int)__reduce_add_sync(0xffffffffu, sums);
+            upto += (int)__reduce_add_sync(0xffffffffu, lane < warp ? sums : 0);
+            __syncthreads();  // the next pass's sums
+            if (counting) {
+                total += pass;
+                if (base + kThreads < p.t.num_seqs) continue;
+                counting = false;
+                span = max(1, (int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
+                begin = min(total, span * (int)blockIdx.x);
+                end = min(total, begin + span);
+                if (base > 0) {
+                    base = -kThreads;
+                    continue;
+                }
+            }
+            upto += before;
+            if (begin < end && begin < upto && begin >= upto - units) {
                 ctl.start.seq = base + threadIdx.x;
                 ctl.start.seq_start = upto - units;
                 ctl.start.units = units;
                 ctl.start.s = mine;
             }
             before += pass;
-            if (before > begin) break;
-            base += kThreads;
-            units = 0;
-            if (base + (int)threadIdx.x < p.t.num_seqs) {
-                mine = tree_sequence(p.t, base + threadIdx.x);
-                units = units_of(p.t, mine);
-            }
-            upto = scan(units);
-            __syncthreads();
-            if (lane == 31) ctl.start.sums[warp] = upto;
-            __syncthreads();
-            pass = 0;
-            for (int i = 0; i < kThreads / 32; ++i) {
-                if (i < warp) upto += ctl.start.sums[i];
-                pass += ctl.start.sums[i];
-            }
-            upto += before;
+            if (begin >= end || before > begin) break;
         }
     }
     __syncthreads();
@@ -375,7 +412,7 @@ template <int D> __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_fe
             }
             tc_fence_after();
             if (warp_live) {
-                const bool whole = n == g.tiles, nothing = l == 0.f;
+                const bool whole = g.parts == 1, nothing = l == 0.f;
                 const int64_t part = (int64_t)blockIdx.x * 2 + (j0 == 0 ? 1 : 0);
                 const int64_t out = (int64_t)(g.s.first + node) * p.t.q_heads + g.kv_head * p.t.group + (live ? row - node * p.t.group : 0);
                 const float keep = nothing ? 0.f : whole ? 1.0f / l : 1.f;
@@ -406,7 +443,16 @@ template <int D> __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_fe
                 }
             }
             tc_fence_before();  // the next segment's first value product starts the accumulator anew, behind this warp's next P
-            if (threadIdx.x == 0 && g.parts) p.records[blockIdx.x] = Record{g.s.first, g.kv_head, rows, g.parts};
+            if (g.parts > 1) {
+                __syncwarp();
+                if (lane == 0) {
+                    __threadfence();
+                    if (atomicInc(&p.arrived[g.cta], kSoftmaxWarps * g.parts - 1) == kSoftmaxWarps * g.parts - 1u) {  // the last one's CTA joins
+                        __threadfence();
+                        ctl.join[j0 > 0 && !(j0 + n < g.tiles) ? 0 : 1] = Join{g.s.first, g.kv_head, rows, g.parts, g.cta};
+                    }
+                }
+            }
             if (g.last) break;
         }
     } else if (warp < kQWarp + kQWarps) {
@@ -414,76 +460,107 @@ template <int D> __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_fe
         // A segment is planned once the queries of the one two before it are not needed any more.  By then its last scores have been
         // asked for, and with them the value products of the segment before: no warp has to do with anything before that one, which is three
         // before the planned one, and the ring holds four.
+        // (The way along the span and what is planned next lie in shared memory: there is no room for them beside the queries.)
         const bool plans = warp == kQWarp;
-        Walk walk{};
-        Segment coming;
-        bool more = false;
+        bool more = plans;  // something is planned next
+        auto plan = [&]() {
+            Walk walk = ctl.walk;
+            Segment coming;
+            more = walk.next(p.t, coming);
+            __syncwarp();
+            if (lane == 0) {
+                ctl.walk = walk;
+                ctl.coming = coming;
+            }
+            __syncwarp();
+        };
         auto publish = [&](int k) {
             if (lane == 0) {
-                ctl.seg[k % kSegRing] = coming;
+                ctl.seg[k % kSegRing] = ctl.coming;
                 mbar_arrive(planned(k));
             }
             __syncwarp();
         };
         if (plans) {
-            walk = Walk{begin, end, ctl.start.seq_start, ctl.start.units, span, ctl.start.seq, ctl.start.s};
+            const Walk walk{begin, end, ctl.start.seq_start, ctl.start.units, span, ctl.start.seq, ctl.start.s};
             __syncwarp();
-            walk.next(p.t, coming);
-            publish(0);
-            more = walk.next(p.t, coming);
-            if (more) publish(1);
+            if (lane == 0) ctl.walk = walk;
+            __syncwarp();
+#pragma unroll 1
+            for (int k = 0; k < 2; ++k) {
+                plan();
+                if (more) publish(k);
+            }
         }
         const int tid = threadIdx.x - kQWarp * 32, quads = (p.t.group + 3) / 4;
+        static_assert(kQWarps * 32 % (D / 8) == 0, "a thread's dims");
+        const int c = tid % (D / 8);  // its 8 dims, of whatever token
+        uint64_t turns[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) turns[e] = p.t.freq.turns[c * 4 + e];
         for (int k = 0;; ++k) {
             const Segment &g = segment(k);
             if (!ok) break;
             const int last = g.last, tasks = g.s.nodes * quads * (D / 8), head0 = g.kv_head * p.t.group, first = g.s.first;
-            // A thread takes 8 dims of up to four heads of a drafted token, whose angles are the same.  The loads of a step are
-            // all in flight during the step before; the first ones while the last scores of the segment before are formed.
-            struct Raw {
-                uint4 q[4];
-                int position;
-            } now, next;
-            auto request = [&](int i, Raw &x) {
-                const int c = i % (D / 8), nq = i / (D / 8), node = nq / quads, h = nq % quads * 4;
-                x.position = p.t.positions[first + node];
-                const char *from = static_cast<const char *>(p.t.q) + (((int64_t)(first + node) * p.t.q_heads + head0 + h) * D + c * 8) * 2;
+            // A thread takes 8 dims of up to four heads of a drafted token, whose angles are the same, kQSteps tokens' at a time: all
+            // loads of 64 rows (of groups of four) are in flight while the last scores of the segment before are formed.
+            uint4 raw[kQSteps][4];
+            int position[kQSteps];
+            auto request = [&](int base) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (h + e < p.t.group) x.q[e] = *reinterpret_cast<const uint4 *>(from + e * D * 2);
+                for (int u = 0; u < kQSteps; ++u) {
+                    const int i = base + u * kQWarps * 32;
+                    if (i >= tasks) break;
+                    const int nq = i / (D / 8), node = quads == 1 ? nq : nq / quads, h = (nq - node * quads) * 4;
+                    position[u] = p.t.positions[first + node];
+                    const char *from = static_cast<const char *>(p.t.q) + (((int64_t)(first + node) * p.t.q_heads + head0 + h) * D + c * 8) * 2;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (h + e < p.t.group) raw[u][e] = *reinterpret_cast<const uint4 *>(from + e * D * 2);
+                }
             };
-            if (tid < tasks) request(tid, now);
-            for (int i = tid; i < g.rows * C::kBoxes; i += kQWarps * 32) {  // the later steps', 128 bytes each
-                const int r = i / C::kBoxes, node = r / p.t.group;
-                const char *at = static_cast<const char *>(p.t.q) + ((int64_t)(first + node) * p.t.q_heads + head0 + r - node * p.t.group) * (D * 2) + i % C::kBoxes * 128;
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
-            }
+            if (k > 0 && more) plan();
+            request(tid);
             if (k > 0) {
-                if (plans && more) more = walk.next(p.t, coming);
                 if (!mbar_wait_warp(q_empty, (k - 1) & 1, abort_flag)) {
                     if (lane == 0) record_timeout(p, 330);
                     ok = false;
                     break;
                 }
-                if (plans && more) publish(k + 1);
+                if (more) publish(k + 1);
+            } else {
+                // The ring's first filling is 24 MB of the whole device: the first queries would arrive behind it, 7000 clk later.
+                uint32_t seen = 0;
+                if (tid < tasks) asm volatile("mov.b32 %0, %1;" : "=r"(seen) : "r"(raw[0][0].x));
+                __syncwarp();
+                if (lane == 0) mbar_arrive(go);
             }
 #pragma unroll 1
-            for (int i = tid; i < tasks; i += kQWarps * 32) {
-                if (i + kQWarps * 32 < tasks) request(i + kQWarps * 32, next);
-                const int c = i % (D / 8), nq = i / (D / 8), node = nq / quads, h = nq % quads * 4;
+            for (int i = tid, step = 0; i < tasks; i += kQWarps * 32) {
+                const int nq = i / (D / 8), node = quads == 1 ? nq : nq / quads, h = (nq - node * quads) * 4;
                 float2 cs[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    cs[e] = turn_of_fast(now.position, ctl.turns[c * 4 + e]);
+                    cs[e] = turn_of_fast(position[0], turns[e]);
                     cs[e].x *= p.t.scale * kLog2e;
                     cs[e].y *= p.t.scale * kLog2e;
                 }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = node * p.t.group + h + e;
-                    if (h + e < p.t.group) write_query<C::kQTile>(now.q[e], cs, q_s + (c >> 3) * C::kQBox + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+#pragma unroll 1
+                for (int r = node * p.t.group + h, e = h; e < min(h + 4, p.t.group); ++e, ++r) {
+                    write_query<C::kQTile>(raw[0][0], cs, q_s + (c >> 3) * C::kQBox + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                    raw[0][0] = raw[0][1], raw[0][1] = raw[0][2], raw[0][2] = raw[0][3];  // registers move so that the loops stay loops
                 }
-                now = next;
+                if (++step == kQSteps) {
+                    step = 0;
+                    request(i + kQWarps * 32);
+                } else {
+#pragma unroll
+                    for (int u = 0; u + 1 < kQSteps; ++u) {
+                        position[u] = position[u + 1];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) raw[u][e] = raw[u + 1][e];
+                    }
+                }
             }
             fence_proxy_async();
             __syncwarp();
@@ -503,6 +580,11 @@ template <int D> __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_fe
             if (!ok) break;
             BoxRows rows;
             rows.start(p.t, g.seq, g.s.tokens, g.j0 * kTok, p.box_rows);
+            if (k == 0 && !mbar_wait_warp(go, 0, abort_flag)) {
+                if (lane == 0) record_timeout(p, 110);
+                ok = false;
+                break;
+            }
             for (int i = 0; i < g.n; ++i, ++count) {
                 const int first = (g.j0 + i) * boxes;
                 rows.seek(first);
@@ -573,28 +655,30 @@ template <int D> __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_fe
                 tc_commit(empty(s));
                 if (i + 1 == n) tc_commit(q_empty);
             };
+            auto values = [&](int v, const Segment &g) {
+                const int b = (done + v) & 1, s = landed(v_entry(v, g.n, kAhead));
+                if (is_tail(g, g.j0 + v)) {
+                    wait(fixed(s), (fixed_phase >> s) & 1, 230);
+                    fixed_phase ^= 1u << s;
+                }
+                wait(p_full(b), ((done + v) >> 1) & 1, 240 + b);
+                if (!ok) return;
+                tc_fence_after();
+#pragma unroll
+                for (int e = 0; e < kTok / 16; ++e)
+                    mma_values<C::kGroup>(tmem_base, tmem_base + col_s(b) + e * 8, v_desc + s * kTile16 + e * (2 * C::kGroup >> 4), p.idesc_pv, v > 0 || e > 0);
+                tc_commit(pv_done(b));
+                tc_commit(empty(s));
+            };
             for (int k = 0;; ++k) {
                 wait(planned(k), (k / kSegRing) & 1, 506);
                 wait(q_ready, k & 1, 200);
                 if (!ok) break;
                 const Segment g = ctl.seg[k % kSegRing];
-                for (int i = 0; i < min(g.n, kAhead); ++i) scores(i, g.n);
-                for (int v = 0; ok && v < g.n; ++v) {
-                    const int b = (done + v) & 1, s = landed(v_entry(v, g.n, kAhead));
-                    if (is_tail(g, g.j0 + v)) {
-                        wait(fixed(s), (fixed_phase >> s) & 1, 230);
-                        fixed_phase ^= 1u << s;
-                    }
-                    wait(p_full(b), ((done + v) >> 1) & 1, 240 + b);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int e = 0; e < kTok / 16; ++e)
-                        mma_values<C::kGroup>(tmem_base, tmem_base + col_s(b) + e * 8, v_desc + s * kTile16 + e * (2 * C::kGroup >> 4), p.idesc_pv,
-                                              v > 0 || e > 0);
-                    tc_commit(pv_done(b));
-                    tc_commit(empty(s));
-                    if (v + kAhead < g.n) scores(v + kAhead, g.n);
+#pragma unroll 1
+                for (int i = 0; ok && i < g.n + kAhead; ++i) {
+                    if (i >= kAhead) values(i - kAhead, g);
+                    if (i < g.n) scores(i, g.n);
                 }
                 if (!ok || g.last) break;
                 done += g.n;
@@ -640,43 +724,12 @@ template <int D> __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_fe
         tc_fence_after();
         tmem_dealloc(tmem_base, 512 / kCtasPerSm);
     }
-}
-
-// Joins the parts of an item that begins in CTA blockIdx.x and ends in a later one, in CTA order: 32 rows a block, a row a lane, D / 8
-// dims a warp.
-template <int D> __global__ void __launch_bounds__(256) tree_few_merge_kernel(const __grid_constant__ KernelParams p) {
-    grid_dependency_wait();
-    grid_dependency_launch();
-    const Record rec = p.records[blockIdx.x];
-    const int warp = threadIdx.x >> 5, r = blockIdx.y * 32 + (threadIdx.x & 31);
-    if (rec.parts <= 0 || r >= rec.rows) return;
-    constexpr int kPer = D / 32;  // groups of four dims
-    auto part = [&](int i) { return (int64_t)((blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)); };
-    float mx = -INFINITY;
-#pragma unroll 4
-    for (int i = 0; i < rec.parts; ++i) mx = fmaxf(mx, p.part_ml[part(i) * kRows + r].x);
-    float sum = 0.f;
-    float4 o[kPer] = {};
-#pragma unroll 2
-    for (int i = 0; i < rec.parts; ++i) {
-        const float2 ml = p.part_ml[part(i) * kRows + r];
-        float4 x[kPer];
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) x[e] = p.part_o[(part(i) * (D / 4) + warp * kPer + e) * kRows + r];
-        if (ml.y == 0.f) continue;  // a part in which the row has seen nothing; a NaN counts
-        const float f = ex2(ml.x - mx);
-        sum = fmaf(f, ml.y, sum);
-#pragma unroll
-        for (int e = 0; e < kPer; ++e)
-            o[e] = make_float4(fmaf(f, x[e].x, o[e].x), fmaf(f, x[e].y, o[e].y), fmaf(f, x[e].z, o[e].z), fmaf(f, x[e].w, o[e].w));
-    }
-    const bool nothing = sum == 0.f;
-    const float inv = nothing ? 0.f : 1.0f / sum;
-    const int64_t out = (int64_t)(rec.first + r / p.t.group) * p.t.q_heads + rec.kv_head * p.t.group + r % p.t.group;
-    uint2 *to = reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p.t.o) + out * D + warp * (D / 8));
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) to[e] = make_uint2(pack_bf16(o[e].x * inv, o[e].y * inv), pack_bf16(o[e].z * inv, o[e].w * inv));
-    if (warp == 0) p.t.lse[out] = nothing ? -INFINITY : (mx + log2f(sum)) * kLn2;
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i)
+        if (ctl.join[i].parts) {
+            join_parts<D>(p, ctl.join[i], reinterpret_cast<float2 *>(q_s));  // queries and ring are done with
+            __syncthreads();  // the next one's statistics
+        }
 }
 
 template <int D> int launch(flat_ctx *ctx, const TreeParams &t) {
@@ -693,26 +746,26 @@ template <int D> int launch(flat_ctx *ctx, const TreeParams &t) {
     char *at = static_cast<char *>(ctx->paged_scratch) + kPagedPlanBytes;
     const uint64_t rows_held = (uint64_t)grid * 2 * kRows;
     const uint64_t o_bytes = rows_held * D * sizeof(float), ml_bytes = rows_held * sizeof(float2);
-    if (o_bytes + ml_bytes + grid * sizeof(Record) > kPagedScratchBytes - kPagedPlanBytes)
+    if (o_bytes + ml_bytes > kPagedScratchBytes - kPagedPlanBytes || (uint64_t)grid > kPagedTickets)
         return fail(ctx, FLAT_ERR_EXECUTION, "the scratch does not hold the parts of %d CTAs", grid);
     p.part_o = reinterpret_cast<float4 *>(at);
     p.part_ml = reinterpret_cast<float2 *>(at + o_bytes);
-    p.records = reinterpret_cast<Record *>(at + o_bytes + ml_bytes);
+    p.arrived = paged_tickets(ctx) + 1;
     FLAT_CUDA_OK(ctx, cudaFuncSetAttribute(tree_few_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     {
         KernelTimer timer(ctx);
         FLAT_CUDA_OK(ctx, launch_dependent(may_overlap_previous(ctx), tree_few_kernel<D>, dim3((unsigned)grid), kThreads, C::kSmem, ctx->stream, p));
     }
     ctx->launches += 1;
-    const int chunks = (int)(((int64_t)t.max_nodes * t.group + 31) / 32);
-    FLAT_CUDA_OK(ctx, launch_dependent(true, tree_few_merge_kernel<D>, dim3((unsigned)grid, (unsigned)chunks), 256, 0, ctx->stream, p));
-    ctx->launches += 1;
     return FLAT_OK;
 }
 
 }  // namespace
 
-bool tree_few_supported(const TreeParams &p) { return (int64_t)p.max_nodes * p.group <= kRows; }
+// few rows, and a line whose length is a 32-bit number
+bool tree_few_supported(const TreeParams &p) {
+    return (int64_t)p.max_nodes * p.group <= kRows && (int64_t)p.kv_heads * p.num_seqs < (1ll << 30) / ((p.max_context + kTok - 1) / kTok);
+}
 
 int launch_tree_few(flat_ctx *ctx, const TreeParams &p) { return p.head_dim == 128 ? launch<128>(ctx, p) : launch<64>(ctx, p); }
 

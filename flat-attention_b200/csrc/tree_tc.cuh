@@ -183,8 +183,8 @@ __device__ __forceinline__ void add_not_finite(const TreeParams &p, const TreeSe
     }
 }
 
-__device__ __forceinline__ int64_t quotient(int64_t x, int d) {  // x >= 0; in 32 bits where they hold it
-    return x >> 32 ? x / d : (int64_t)((uint32_t)x / (uint32_t)d);
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t d) {  // x >= 0, d > 0; in 32 bits where they hold both
+    return (x | d) >> 32 ? x / d : (int64_t)((uint32_t)x / (uint32_t)d);
 }
 
 // 5-D map over (64 dims, token of 8, 64-dim block, group of 8 tokens, head) of a pool, with a box of one head's `box_rows` tokens.
