@@ -2043,7 +2043,7 @@ int32_t flat_decode_paged_tree(flat_ctx *ctx, int32_t dtype, const flat_paged_ba
     p.scale = scale;
     p.status = ctx->dev_status;
     fill_turns(ctx, theta, p.head_dim, &p.freq);
-    if (tree_sm100_supported(dtype, p)) return tree_few_supported(p) ? launch_tree_few(ctx, p) : launch_tree_sm100(ctx, p);
+    if (tree_sm100_supported(dtype, p)) return launch_tree_sm100(ctx, p);
     return launch_tree_simt(ctx, dtype, p);
 }
 

@@ -380,8 +380,6 @@ int launch_tree_simt(flat_ctx *ctx, int dtype, TreeParams &p);
 // bf16, head_dim 64 or 128, pages of a multiple of 16 tokens, 16-byte aligned buffers
 bool tree_sm100_supported(int dtype, const TreeParams &p);
 int launch_tree_sm100(flat_ctx *ctx, const TreeParams &p);
-bool tree_few_supported(const TreeParams &p);  // where tree_sm100_supported
-int launch_tree_few(flat_ctx *ctx, const TreeParams &p);
 
 // ---- backward --------------------------------------------------------------------------------
 struct BwdParams {

@@ -3,20 +3,23 @@
 //   rows of one (sequence, KV head): (drafted token, head of the group), n * G of them, all against the same keys and values
 //   S = Q K^T (SS MMA, 128 rows x 64 tokens)  ->  P = exp2(S - m)  ->  O += P V (A operand from TMEM)
 //
-// The bytes are those of K and V, read once; with many drafted tokens the products cost as much, so both are kept going at once: two
-// warps stream tiles of 128 tokens by TMA, a box per page or tile, into a ring whatever item is at hand; one thread issues all
-// products; two groups of four warps ("slots") each own a 128-row accumulator and work a softmax row per thread, without shuffles.
-//   more than 128 rows: slot w has rows 128 w .. and both slots take every tile, which crosses into the SM once for 256 rows;
-//   otherwise:          both slots have the same rows and take the tiles in turn, and their states are joined at the end.  A slot is
-//                       a chain (scores, softmax, values), and one alone does not keep up with the memory.
-// P lies over the scores it comes from; the products of one thread execute in order, so the next scores of a slot cannot overtake
-// the product that reads its P, and a slot that sees its scores knows that its last value product is complete.  Tiles of 64 tokens
-// with two score tiles a slot were slower: the queries cross from shared memory for every tile, which at 64 tokens takes the tensor
-// core longer than the product (a product of 128 x 64 x 16 every 46 clk, of 128 x 128 x 16 every 64).
+// Bound by the bytes of K and V, read once, and with hundreds of rows by the products; either way what counts is that nothing stands between
+// two tiles.  The beginning and the end of an item (queries read, turned and written; the first scores; the last weights; results) are
+// a chain of 10000 clk and more, and a load takes 2000 clk while K and V stream in.  So:
+//   two CTAs share an SM, 112 KB and half the TMEM each;
+//   K and V tiles of 64 tokens come by TMA, a box per page or tile, through a ring that runs on whatever item is at hand;
+//   one warp plans: it walks the span two items ahead of the products and puts what the other warps have to know in shared memory;
+//   two warps make the next item's queries as soon as the last scores of the item before are formed;
+//   ROWS / 32 warps work a softmax row per thread, without shuffles, and write results, while the next item's first scores are formed;
+//   one thread issues all products.  Two score tiles alternate; P lies over the scores it comes from, and the products of one
+//   thread execute in order, so the scores after next cannot overtake the product that reads that P.
+// ROWS is 64 where no sequence has more (the ring takes the queries' place; half the rows of a product are whatever lies behind the
+// queries in shared memory: a product of 64 rows takes as long), otherwise 128.  Of more than 128 rows, two blocks of 128 go to two CTAs
+// that walk the same span, so that the second one finds K and V in the L2.
 //
-// Work: the tiles of all (sequence, KV head, 256 rows) items stand in one line, which is cut into equal spans, one per CTA, whatever
+// Work: the tiles of all items, a block of ROWS rows of a (sequence, KV head) each, stand in one line, which is cut into equal spans, one per CTA, whatever
 // the lengths are.  Every CTA adds the lengths up itself, so nothing is planned on the host.  An item that a span's end cuts is
-// joined by a small second kernel from the parts, in order; everything else is written directly.
+// joined, from the parts in order, by the CTA that finds that they are all there; everything else is written directly.
 //
 // Roundings: q enters as the sum of two bf16 numbers (the tensor core takes one type, and K is bf16; q alone would cost 2^-9 of the
 // scores: 1.7 times the error of the bf16 result, where this way is 1.4 times it), P as bf16, sums and statistics are f32.
@@ -27,98 +30,98 @@
 // warp goes over the V tiles that hold drafted tokens or the end of a sequence before they are used: rows behind the end (whatever
 // an earlier owner of the page left) become zero, and so do values of drafted tokens that are not finite; these are then added to
 // the rows that see them at the end, where they were met at all.
-#include <cuda.h>
-
-#include "common.h"
-#include "sm100_host.cuh"
-#include "sm100_ptx.cuh"
-#include "tree.cuh"
-#include "turns.cuh"
+#include "tree_tc.cuh"
 
 namespace flat {
 namespace {
 
-using namespace sm100;
+using namespace tree_tc;
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kRescaleThreshold = 8.0f;  // log2 domain
-constexpr int kTok = 128, kSlotRows = 128, kItemRows = 2 * kSlotRows;
-constexpr int kSoftmaxWarps = 8, kKWarp = 8, kVWarp = 9, kMmaWarp = 10;  // ... and one that goes over V tiles
-constexpr int kThreads = 384;
+constexpr int kTok = 64, kAhead = 2;  // kAhead: score tiles
+constexpr int kQWarps = 2, kCtasPerSm = 2;
+constexpr int kSegRing = 4;      // see below, planning
 constexpr int kValidRing = 16;   // tiles between the producer and the slowest softmax warp: the ring's and four more
 constexpr int kPoisonRing = 16;  // segments between the fixing warp and the slowest softmax warp
-constexpr int kMergeChunks = 8;  // blocks per item, 32 rows each
 
-// NARROW: no item has more than 128 rows; the ring takes the second slot's queries' place.
 // A K or V tile lies in shared memory as [8 tokens][64 dims of D][token of the 8][64 dims]: one TMA box of any number of tokens
-// then writes all D dims.
-template <int D, bool NARROW> struct Cfg {
+// then writes all D dims.  Queries: [summand][64 dims of D][row][64 dims].
+template <int D, int ROWS> struct Cfg {
+    static constexpr int kSoftmaxWarps = ROWS / 32, kQWarp = kSoftmaxWarps, kKWarp = kQWarp + kQWarps, kVWarp = kKWarp + 1, kMmaWarp = kVWarp + 1;
+    static constexpr int kThreads = (kMmaWarp + 2) * 32;  // the last warp goes over V tiles
+    static constexpr int kQSteps = ROWS == 64 ? 4 : 2;    // tokens of a thread of the query warps in flight
     static constexpr int kBoxes = D / 64;
-    static constexpr int kQBox = kSlotRows * 128, kQTile = kQBox * kBoxes;  // one of the two summands of a slot's queries
-    static constexpr int kGroup = 1024 * kBoxes;                            // 8 tokens
+    static constexpr int kQBox = ROWS * 128, kQTile = kQBox * kBoxes;  // one of the two summands of the queries
+    static constexpr int kGroup = 1024 * kBoxes;                        // 8 tokens
     static constexpr int kKvTile = kTok / 8 * kGroup;
-    static constexpr int kQBytes = (NARROW ? 2 : 4) * kQTile;
-    static constexpr int kStages = (224 * 1024 - kQBytes) / kKvTile;  // D = 128: 5 and 3, D = 64: 12 and 10
-    static constexpr int kSmem = kQBytes + kStages * kKvTile + 1024;
+    static constexpr int kControl = 1024, kSmem = (228 / kCtasPerSm - 1) * 1024;  // of an SM's 228 KB, 1 KB a CTA is the system's
+    static constexpr int kStages = (kSmem - kControl - 2 * kQTile) / kKvTile;     // D = 128: 5 and 3, D = 64: 12 and 10
+    static_assert(2 * kQTile - kQBox + kMmaRows * 128 <= 2 * kQTile + kStages * kKvTile, "what a product reads behind the queries");
 };
 
-struct Record {  // an item that begins in this CTA and ends in a later one
-    int seq, kv_head, pair, parts;
-};
 struct KernelParams {
     TreeParams t;
     CUtensorMap map_k, map_v;
     uint32_t idesc_qk, idesc_pv;
-    int box_rows;      // tokens of a TMA box: 16, 32, 64 or 128, a divisor of the page size
-    float *part_o;     // [2 per CTA][256 rows][D], not normalised
-    float2 *part_ml;   // [2 per CTA][256 rows] maximum (log2 domain) and sum
-    Record *records;   // [CTA]
+    int box_rows;      // tokens of a TMA box: 16, 32 or 64, a divisor of the page size
+    int share;         // CTAs of a span: 2 where two blocks of rows share K and V
+    float4 *part_o;    // [2 per CTA][D / 4][ROWS], not normalised
+    float2 *part_ml;   // [2 per CTA][ROWS] maximum (log2 domain) and sum
+    unsigned *arrived; // [CTA]: warps that have written their part of the item that begins in this CTA and ends in a later one; 0 between calls
 };
 
 // A part of an item that one CTA works on.
 struct Segment {
     TreeSequence s;
-    int seq, kv_head, pair;  // pair: which 256 rows
-    int rows;                // of the pair
-    int j0, j1, tiles;       // its tiles, and the item's
-    int64_t item_end;        // on the line
+    int seq, kv_head;
+    int row0, rows;    // of the (sequence, KV head)
+    int j0, n, tiles;  // its first tile, its tiles (0: there are no more segments), the item's
+    int parts, cta;    // of an item that is cut, and the CTA that it begins in; otherwise parts = 1
 };
 
-__device__ __forceinline__ int64_t units_of(const TreeParams &p, const TreeSequence &s) {
-    if (s.nodes == 0) return 0;
-    const int64_t pairs = ((int64_t)s.nodes * p.group + kItemRows - 1) / kItemRows;
-    return pairs * p.kv_heads * max(1, (s.tokens + kTok - 1) / kTok);
+__device__ __forceinline__ int tiles_of(const TreeSequence &s) { return max(1, (s.tokens + kTok - 1) / kTok); }
+template <int ROWS> __device__ __forceinline__ int blocks_of(const TreeParams &p, const TreeSequence &s) { return (s.nodes * p.group + ROWS - 1) / ROWS; }
+// What a sequence takes of the line: the tiles of its items, or of its pairs of items where two CTAs walk a span.
+template <int ROWS> __device__ __forceinline__ int units_of(const KernelParams &p, const TreeSequence &s) {
+    return s.nodes == 0 ? 0 : (blocks_of<ROWS>(p.t, s) * p.t.kv_heads + p.share - 1) / p.share * tiles_of(s);
 }
 
-// A CTA's walk over its span; every role makes it for itself.
-struct Walk {
-    int64_t at, end, seq_start;
-    int seq;
-    __device__ __forceinline__ bool next(const TreeParams &p, Segment &g) {
+// A CTA's way along its span.
+template <int ROWS> struct Walk {
+    int at, end, seq_start, units, span, seq;
+    TreeSequence s;  // of seq
+    __device__ __forceinline__ void next(const KernelParams &p, Segment &g) {
+        g.n = 0;
         while (at < end) {
-            const TreeSequence s = tree_sequence(p, seq);
-            const int64_t units = units_of(p, s);
             if (at >= seq_start + units) {
                 seq_start += units;
-                ++seq;
+                s = tree_sequence(p.t, ++seq);
+                units = units_of<ROWS>(p, s);
                 continue;
             }
-            const int tiles = max(1, (s.tokens + kTok - 1) / kTok);
-            const int64_t x = at - seq_start, item = x / tiles;
-            const int pairs = (int)(((int64_t)s.nodes * p.group + kItemRows - 1) / kItemRows);
+            const int tiles = tiles_of(s), blocks = blocks_of<ROWS>(p.t, s);
+            const int pair = (int)((unsigned)(at - seq_start) / (unsigned)tiles), item_start = seq_start + pair * tiles;
+            const int lane = p.share == 2 ? (int)blockIdx.x & 1 : 0, item = pair * p.share + lane;
+            const int j0 = at - item_start, n = min(tiles - j0, end - at);
+            at += n;
+            const int kv_head = (int)((unsigned)item / (unsigned)blocks);
+            if (kv_head >= p.t.kv_heads) continue;  // an odd number of items: nothing for the second CTA
             g.s = s;
             g.seq = seq;
-            g.kv_head = (int)(item / pairs);
-            g.pair = (int)(item % pairs);
-            g.rows = min(kItemRows, s.nodes * p.group - g.pair * kItemRows);
+            g.kv_head = kv_head;
+            g.row0 = (item - kv_head * blocks) * ROWS;
+            g.rows = min(ROWS, s.nodes * p.t.group - g.row0);
             g.tiles = tiles;
-            g.j0 = (int)(x - item * tiles);
-            g.j1 = (int)min((int64_t)tiles, g.j0 + (end - at));
-            g.item_end = seq_start + (item + 1) * tiles;
-            at += g.j1 - g.j0;
-            return true;
+            g.j0 = j0;
+            g.n = n;
+            g.parts = 1;
+            g.cta = blockIdx.x;
+            if (n < tiles) {
+                const int first = (int)((unsigned)item_start / (unsigned)span);
+                g.cta = first * p.share + lane;
+                g.parts = (int)((unsigned)(item_start + tiles - 1) / (unsigned)span) - first + 1;
+            }
+            return;
         }
-        return false;
     }
 };
 
@@ -127,531 +130,470 @@ __device__ __forceinline__ void record_timeout(const KernelParams &p, int where)
     p.t.status->where = where;
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 // Whether tile j of the segment's item holds drafted tokens or is its last: its V tile is gone over before it is used.  (Every
 // item has such a tile, so the warp that does it is never more than the ring ahead.)
 __device__ __forceinline__ bool is_tail(const Segment &g, int j) { return (j + 1) * kTok > g.s.len || j + 1 == g.tiles; }
 
-// Which of the 64 tokens from t0 on drafted token `node` sees; valid: 16-token groups whose page is in the pool (4 bits).
-__device__ __forceinline__ uint64_t visible(const TreeParams &p, const TreeSequence &s, int node, int t0, uint32_t valid) {
-    auto ones = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
-    const uint64_t live = ones(s.len - t0);
-    uint64_t drafts = 0;
-    if (t0 + 64 > s.len) {
-        const int j = t0 - s.len;  // drafted token of the first column, if not negative
-        if (!p.mask) {
-            drafts = p.causal ? ones(node - j + 1) : ~0ull;
-        } else {
-            const uint32_t *row = p.mask + (int64_t)(s.first + node) * p.mask_words;
-            auto word = [&](int i) { return i < p.mask_words ? (uint64_t)row[i] : 0ull; };
-            if (j <= 0) {
-                drafts = (word(0) | word(1) << 32) << -j;  // -j < 64
-            } else {
-                const int w = j >> 5, shift = j & 31;
-                drafts = (word(w) | word(w + 1) << 32) >> shift;
-                if (shift) drafts |= word(w + 2) << (64 - shift);
-            }
-        }
-    }
-    uint64_t on = (live | (drafts & ~live)) & ones(s.tokens - t0);
-    if (valid != 0xf)
-        for (int i = 0; i < 4; ++i)
-            if (!((valid >> i) & 1)) on &= ~(0xffffull << (16 * i));
-    return on;
-}
-
-// D[tmem] (+)= A B^T with both operands in shared memory, 128-byte swizzle, rows in groups of 8: A's groups 1024 bytes apart, B's B_SBO.
-template <int B_SBO>
-__device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        ".reg .b64 da, db;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "mov.b64 da, {%1, %5};\n"
-        "mov.b64 db, {%2, %6};\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
-        "}\n" ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"((1024 >> 4) | (1 << 14) | (2 << 29)),
-        "n"((B_SBO >> 4) | (1 << 14) | (2 << 29))
-        : "memory");
-}
-template <int B_SBO>
-__device__ __forceinline__ void mma_values(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        ".reg .b64 db;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "mov.b64 db, {%2, %5};\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n"
-        "}\n" ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"((B_SBO >> 4) | (1 << 14) | (2 << 29))
-        : "memory");
-}
-
-__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap *map, int group, int head, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3, %4}], [%5];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(group), "r"(head), "r"(bar)
-        : "memory");
-}
-
-// Order of the tiles of a segment of n tiles in the ring: the first `ahead` K tiles, then V tile v and K tile v + ahead for each v.
-__device__ __forceinline__ int k_entry(int i, int ahead) { return i < ahead ? i : 2 * i - ahead + 1; }
-__device__ __forceinline__ int v_entry(int v, int n, int ahead) { return min(n, ahead) + v + min(v, max(0, n - ahead)); }
-
-// The pool rows of a sequence's boxes, 32 at a time, a box per lane, the next 32 on their way.
-struct BoxRows {
-    const int32_t *table;
-    int page_size, box_rows, tokens, base, lane;
-    int page, in_page, page_next, in_page_next;
-    __device__ __forceinline__ void fetch(int box, int &to, int &in) {
-        const int t = box * box_rows;
-        to = -2;  // nothing to read: zeros
-        in = 0;
-        if (t < tokens) {
-            const int logical = t / page_size;
-            to = max(table[logical], -1);
-            in = t - logical * page_size;
-        }
-    }
-    __device__ __forceinline__ void start(const TreeParams &p, const Segment &g, int rows) {
-        lane = threadIdx.x & 31;
-        table = p.page_tables + (int64_t)g.seq * p.max_pages;
-        page_size = p.page_size;
-        box_rows = rows;
-        tokens = g.s.tokens;
-        base = g.j0 * (kTok / rows);
-        fetch(base + lane, page, in_page);
-        fetch(base + 32 + lane, page_next, in_page_next);
-    }
-    __device__ __forceinline__ void seek(int box) {  // boxes are asked for in order, a tile's at a time
-        if (box - base < 32) return;
-        base += 32;
-        page = page_next;
-        in_page = in_page_next;
-        fetch(base + 32 + lane, page_next, in_page_next);
-    }
+struct Join {  // an item whose parts are all there
+    int first, kv_head, row0, rows, parts, cta;
 };
 
-template <int D, bool NARROW> __global__ void __launch_bounds__(kThreads, 1) tree_sm100_kernel(const __grid_constant__ KernelParams p) {
-    using C = Cfg<D, NARROW>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *q_s = smem;                // [slot][summand]; at the end of a segment, results on their way out
-    uint8_t *kv_s = smem + C::kQBytes;  // ring
-    __shared__ uint64_t bars[4 * C::kStages + 9];
-    __shared__ uint64_t turns_s[D / 2];
-    __shared__ uint32_t tmem_slot[1];
-    __shared__ int abort_word;
-    __shared__ uint32_t valid_s[kValidRing];
-    __shared__ int poison_s[kPoisonRing];
-    __shared__ int64_t sums_s[kThreads / 32];
-    __shared__ int64_t start_s[2];
-    volatile int *abort_flag = &abort_word;
+// What the warps of a CTA share, at the start of its shared memory.
+template <int ROWS, int STAGES> struct Control {
+    uint64_t bars[4 * STAGES + 9 + kSegRing];
+    union {
+        Segment seg[kSegRing];
+        struct {  // before the first is planned
+            int sums[16];
+            int seq_start, units, seq;
+            TreeSequence s;
+        } start;
+    };
+    uint32_t tmem;
+    int abort;
+    Walk<ROWS> walk;  // of the planning warp
+    Segment coming;
+    Join join[2];  // an item that ends here, and one that does not
+    uint8_t valid[kValidRing], poison[kPoisonRing];
+};
 
-    const uint32_t bar0 = smem_u32(bars);
+// Joins the parts of an item in CTA order, whichever came last: a row a thread and a share of the dims.
+template <int D, int ROWS> __device__ __forceinline__ void join_parts(const KernelParams &p, const Join &item) {
+    const int lanes = item.rows <= 32 ? 32 : item.rows <= 64 ? 64 : 128, r = threadIdx.x & (lanes - 1), g = threadIdx.x / lanes, groups = 256 / lanes;
+    const int parts = item.parts;
+    if (r >= item.rows || threadIdx.x >= 256) return;
+    auto part = [&](int i) { return (int64_t)((item.cta + i * p.share) * 2 + (i == 0 ? 1 : 0)); };  // the first CTA's second, the others' first
+    auto weight = [](float2 ml, float mx) { return ml.y == 0.f ? 0.f : ex2(ml.x - mx); };  // a part in which the row has seen nothing; a NaN counts
+    float mx = -INFINITY, sum = 0.f;
+#pragma unroll 1
+    for (int base = 0; base < parts; base += 4) {
+        float2 ml[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) ml[u] = base + u < parts ? __ldcg(&p.part_ml[part(base + u) * ROWS + r]) : make_float2(-INFINITY, 0.f);
+        const float before = mx;
+        mx = fmaxf(fmaxf(mx, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+        sum *= before == -INFINITY ? 0.f : ex2(before - mx);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum = fmaf(weight(ml[u], mx), ml[u].y, sum);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const int row = item.row0 + r, node = row / p.t.group;
+    const int64_t out = (int64_t)(item.first + node) * p.t.q_heads + item.kv_head * p.t.group + row - node * p.t.group;
+    if (g == 0) p.t.lse[out] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+#pragma unroll 1
+    for (int d4 = g * 4; d4 < D / 4; d4 += groups * 4) {
+        float4 o[4] = {};
+#pragma unroll 1
+        for (int base = 0; base < parts; base += 2) {
+            float4 x[2][4];
+            float2 ml[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                if (base + u < parts) {
+                    ml[u] = __ldcg(&p.part_ml[part(base + u) * ROWS + r]);
+                    const float4 *from = p.part_o + (part(base + u) * (D / 4) + d4) * ROWS + r;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[u][e] = __ldcg(from + e * ROWS);
+                }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                if (base + u < parts) {
+                    const float f = weight(ml[u], mx) * inv;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        o[e] = make_float4(fmaf(f, x[u][e].x, o[e].x), fmaf(f, x[u][e].y, o[e].y), fmaf(f, x[u][e].z, o[e].z), fmaf(f, x[u][e].w, o[e].w));
+                }
+        }
+        uint4 *to = reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.t.o) + out * D + d4 * 4);
+        to[0] = make_uint4(pack_bf16(o[0].x, o[0].y), pack_bf16(o[0].z, o[0].w), pack_bf16(o[1].x, o[1].y), pack_bf16(o[1].z, o[1].w));
+        to[1] = make_uint4(pack_bf16(o[2].x, o[2].y), pack_bf16(o[2].z, o[2].w), pack_bf16(o[3].x, o[3].y), pack_bf16(o[3].z, o[3].w));
+    }
+}
+
+template <int D, int ROWS>
+__global__ void __launch_bounds__((ROWS / 32 + 6) * 32, kCtasPerSm) tree_sm100_kernel(const __grid_constant__ KernelParams p) {
+    using C = Cfg<D, ROWS>;
+    using Ctl = Control<ROWS, C::kStages>;
+    constexpr int kSoftmaxWarps = C::kSoftmaxWarps, kQWarp = C::kQWarp, kKWarp = C::kKWarp, kVWarp = C::kVWarp, kMmaWarp = C::kMmaWarp;
+    constexpr int kThreads = C::kThreads, kQSteps = C::kQSteps;
+    static_assert(kThreads == (ROWS / 32 + 6) * 32, "launch bounds");
+    extern __shared__ __align__(1024) uint8_t smem[];
+    Ctl &ctl = *reinterpret_cast<Ctl *>(smem);
+    static_assert(sizeof(Ctl) <= C::kControl, "control block");
+    uint8_t *q_s = smem + C::kControl;       // [summand]
+    uint8_t *kv_s = q_s + 2 * C::kQTile;     // ring
+    volatile int *abort_flag = &ctl.abort;
+
+    const uint32_t bar0 = smem_u32(ctl.bars);
     auto full = [&](int s) { return bar0 + 8u * s; };                        // tile landed
     auto empty = [&](int s) { return bar0 + 8u * (C::kStages + s); };        // tile used
     auto fixed = [&](int s) { return bar0 + 8u * (2 * C::kStages + s); };    // V tile with drafted tokens gone over
     auto to_fix = [&](int s) { return bar0 + 8u * (3 * C::kStages + s); };   // such a tile has been requested
-    auto s_full = [&](int w) { return bar0 + 8u * (4 * C::kStages + w); };       // scores of the slot's tile, and its last value product
-    auto p_full = [&](int w) { return bar0 + 8u * (4 * C::kStages + 2 + w); };   // P written
-    auto o_final = [&](int w) { return bar0 + 8u * (4 * C::kStages + 4 + w); };  // the slot's last value product of the segment
-    const uint32_t q_ready = bar0 + 8u * (4 * C::kStages + 6);    // queries of the segment written
-    const uint32_t q_free = bar0 + 8u * (4 * C::kStages + 7);     // a segment's queries and results are not needed any more
-    const uint32_t join_full = bar0 + 8u * (4 * C::kStages + 8);  // slot 1's statistics written
+    auto s_full = [&](int b) { return bar0 + 8u * (4 * C::kStages + b); };       // scores in tile b
+    auto p_full = [&](int b) { return bar0 + 8u * (4 * C::kStages + 2 + b); };   // P written over tile b
+    auto pv_done = [&](int b) { return bar0 + 8u * (4 * C::kStages + 4 + b); };  // ... and used
+    const uint32_t q_ready = bar0 + 8u * (4 * C::kStages + 6);                   // queries of the segment written
+    const uint32_t q_empty = bar0 + 8u * (4 * C::kStages + 7);                   // ... and not needed any more
+    const uint32_t go = bar0 + 8u * (4 * C::kStages + 8);                        // K and V may be asked for
+    auto planned = [&](int k) { return bar0 + 8u * (4 * C::kStages + 9 + k % kSegRing); };  // segment k
 
     const int warp = warp_index_uniform(), lane = threadIdx.x & 31;
-    grid_dependency_wait();
-    grid_dependency_launch();
     if (threadIdx.x == 0) {
         *abort_flag = 0;
+        ctl.join[0].parts = ctl.join[1].parts = 0;
         for (int s = 0; s < C::kStages; ++s) {
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
             mbar_init(fixed(s), 1);
             mbar_init(to_fix(s), 1);
         }
-        for (int w = 0; w < 2; ++w) {
-            mbar_init(s_full(w), 1);
-            mbar_init(p_full(w), 4);
-            mbar_init(o_final(w), 1);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(s_full(b), 1);
+            mbar_init(p_full(b), kSoftmaxWarps);
+            mbar_init(pv_done(b), 1);
         }
-        mbar_init(q_ready, kSoftmaxWarps);
-        mbar_init(q_free, kSoftmaxWarps);
-        mbar_init(join_full, 4);
+        mbar_init(q_ready, kQWarps);
+        mbar_init(q_empty, 1);
+        mbar_init(go, kQWarps);
+        for (int k = 0; k < kSegRing; ++k) mbar_init(planned(k), 1);
         mbar_fence_init();
         fence_proxy_async();
         tma_prefetch_desc(&p.map_k);
         tma_prefetch_desc(&p.map_v);
     }
-    if (threadIdx.x < kPoisonRing) poison_s[threadIdx.x] = 0;
-    if (threadIdx.x < D / 2) turns_s[threadIdx.x] = p.t.freq.turns[threadIdx.x];
     if (warp == kMmaWarp) {
-        tmem_alloc(smem_u32(tmem_slot), 512);
+        tmem_alloc(smem_u32(&ctl.tmem), 512 / kCtasPerSm);
         tmem_relinquish();
     }
+    grid_dependency_wait();
+    grid_dependency_launch();
 
-    // The line's length, and the sequence that this CTA's span starts in.
-    int64_t total = 0;
-    for (int base = 0; base < p.t.num_seqs; base += kThreads) {
-        const int seq = base + threadIdx.x;
-        if (seq < p.t.num_seqs) {
-            const TreeSequence s = tree_sequence(p.t, seq);
-            total += units_of(p.t, s);
-            if (s.code && blockIdx.x == 0) tree_report(p.t, s.code, seq);
-        }
-    }
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-    if (lane == 0) sums_s[warp] = total;
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    total = 0;
-    for (int i = 0; i < kThreads / 32; ++i) total += sums_s[i];
-    const int64_t span = max((int64_t)1, (total + gridDim.x - 1) / gridDim.x);
-    const int64_t begin = min(total, span * blockIdx.x), end = min(total, begin + span);
-    if (begin < end) {
-        int64_t before = 0;  // units of the sequences of earlier passes
+    // The line's length, then the sequence that this CTA's span starts in: a scan over kThreads sequences at a time, the same once more
+    // where there are more.  (What runs once is kept short here and below: instructions that are not in the cache yet come at a
+    // tenth of the rate.)
+    int span = 1, begin = 0, end = 0;
+    {
+        int total = 0, before = 0;
+        bool counting = true;
+#pragma unroll 1
         for (int base = 0;; base += kThreads) {
-            const int seq = base + threadIdx.x;
-            const int64_t units = seq < p.t.num_seqs ? units_of(p.t, tree_sequence(p.t, seq)) : 0;
-            int64_t upto = units;
+            TreeSequence mine{};
+            int units = 0;
+            if (base + (int)threadIdx.x < p.t.num_seqs) {
+                mine = tree_sequence(p.t, base + threadIdx.x);
+                units = units_of<ROWS>(p, mine);
+                if (mine.code && counting && blockIdx.x == 0) tree_report(p.t, mine.code, base + threadIdx.x);
+            }
+            int upto = units;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
-                const int64_t y = __shfl_up_sync(0xffffffffu, upto, d);
+                const int y = __shfl_up_sync(0xffffffffu, upto, d);
                 if (lane >= d) upto += y;
             }
+            if (lane == 31) ctl.start.sums[warp] = upto;
+            tc_fence_before();
             __syncthreads();
-            if (lane == 31) sums_s[warp] = upto;
-            __syncthreads();
-            int64_t pass = 0;
-            for (int i = 0; i < kThreads / 32; ++i) {
-                if (i < warp) upto += sums_s[i];
-                pass += sums_s[i];
+            tc_fence_after();
+            const int sums = lane < kThreads / 32 ? ctl.start.sums[lane] : 0;
+            const int pass = (int)__reduce_add_sync(0xffffffffu, sums);
+            upto += (int)__reduce_add_sync(0xffffffffu, lane < warp ? sums : 0);
+            __syncthreads();  // the next pass's sums
+            if (counting) {
+                total += pass;
+                if (base + kThreads < p.t.num_seqs) continue;
+                counting = false;
+                const unsigned spans = gridDim.x / p.share, line = blockIdx.x / p.share;
+                span = max(1, (int)((unsigned)(total + spans - 1) / spans));
+                begin = min(total, span * (int)line);
+                end = min(total, begin + span);
+                if (base > 0) {
+                    base = -kThreads;
+                    continue;
+                }
             }
             upto += before;
-            if (begin < upto && begin >= upto - units) {
-                start_s[0] = seq;
-                start_s[1] = upto - units;
+            if (begin < end && begin < upto && begin >= upto - units) {
+                ctl.start.seq = base + threadIdx.x;
+                ctl.start.seq_start = upto - units;
+                ctl.start.units = units;
+                ctl.start.s = mine;
             }
             before += pass;
-            if (before > begin) break;
+            if (begin >= end || before > begin) break;
         }
     }
-    if (threadIdx.x == 0) p.records[blockIdx.x].parts = 0;
     __syncthreads();
-    const uint32_t tmem_base = *tmem_slot;
-    auto col_o = [](int w) { return (uint32_t)(w * D); };
-    auto col_s = [](int w) { return (uint32_t)(2 * D + w * kTok); };
-    Walk walk{begin, end, start_s[1], (int)start_s[0]};
-    Segment g;
+    const uint32_t tmem_base = ctl.tmem;
+    auto col_s = [](int b) { return (uint32_t)(D + b * kTok); };  // O in columns 0 .. D - 1
+    bool ok = true;
+    auto segment = [&](int k) -> const Segment & {  // waits until it is planned
+        if (!mbar_wait_warp(planned(k), (k / kSegRing) & 1, abort_flag)) {
+            if (lane == 0) record_timeout(p, 500 + warp);
+            ok = false;
+        }
+        return ctl.seg[k % kSegRing];
+    };
 
-    if (warp < kSoftmaxWarps) {
-        // ================= queries, softmax, results =================
-        const int w = warp >> 2, row = threadIdx.x & (kSlotRows - 1);
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's quarter of the TMEM lanes
-        int count = 0;      // tiles of this slot so far
-        int tile_base = 0;  // tiles of this CTA before the segment
-        int finals = 0;     // segments in which this slot had tiles
-        int joins = 0;
-        bool ok = true;
-        for (int k = 0; ok && walk.next(p.t, g); ++k) {
-            const bool shared = NARROW || g.rows <= kSlotRows;
-            const int n = g.j1 - g.j0, r_begin = g.pair * kItemRows;
-            {
-                // A thread takes 8 dims of up to four heads of a drafted token, whose angles are the same.  The loads of a step are
-                // all in flight during the step before; the first ones while other warps finish the segment before.
-                const int node_lo = r_begin / p.t.group, node_hi = (r_begin + g.rows - 1) / p.t.group;
-                const int quads = (p.t.group + 3) / 4, tasks = (node_hi - node_lo + 1) * quads * (D / 8);
-                struct Raw {
-                    uint4 q[4];
-                    int position;
-                } now, next;
-                auto request = [&](int i, Raw &x) {
-                    const int c = i % (D / 8), nq = i / (D / 8), node = node_lo + nq / quads, h = nq % quads * 4;
-                    x.position = p.t.positions[g.s.first + node];
-                    const char *from = static_cast<const char *>(p.t.q) +
-                                       (((int64_t)(g.s.first + node) * p.t.q_heads + g.kv_head * p.t.group + h) * D + c * 8) * 2;
-                    const int r = node * p.t.group - r_begin + h;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (h + e < p.t.group && r + e >= 0 && r + e < g.rows) x.q[e] = *reinterpret_cast<const uint4 *>(from + e * D * 2);
-                };
-                if ((int)threadIdx.x < tasks) request(threadIdx.x, now);
-                if (k > 0 && !mbar_wait_warp(q_free, (k - 1) & 1, abort_flag)) {
-                    if (lane == 0) record_timeout(p, 330 + w);
-                    ok = false;
-                    break;
-                }
-                for (int i = threadIdx.x; i < tasks; i += kSoftmaxWarps * 32) {
-                    if (i + kSoftmaxWarps * 32 < tasks) request(i + kSoftmaxWarps * 32, next);
-                    const int c = i % (D / 8), nq = i / (D / 8), node = node_lo + nq / quads, h = nq % quads * 4;
-                    float2 cs[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        cs[e] = turn_of_fast(now.position, turns_s[c * 4 + e]);
-                        cs[e].x *= p.t.scale * kLog2e;
-                        cs[e].y *= p.t.scale * kLog2e;
-                    }
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int r = node * p.t.group - r_begin + h + q;
-                        if (h + q >= p.t.group || r < 0 || r >= g.rows) continue;
-                        const uint32_t x[4] = {now.q[q].x, now.q[q].y, now.q[q].z, now.q[q].w};
-                        uint32_t hi[4], lo[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float a = __uint_as_float(x[e] << 16), b = __uint_as_float(x[e] & 0xffff0000u);
-                            const float u = a * cs[e].x - b * cs[e].y, v = a * cs[e].y + b * cs[e].x;
-                            const __nv_bfloat162 h2 = __floats2bfloat162_rn(u, v);
-                            const float2 f = __bfloat1622float2(h2);
-                            hi[e] = *reinterpret_cast<const uint32_t *>(&h2);
-                            lo[e] = pack_bf16(u - f.x, v - f.y);
-                        }
-                        const int rr = r & (kSlotRows - 1);
-                        uint8_t *to = q_s + (r >> 7) * 2 * C::kQTile + (c >> 3) * C::kQBox + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
-                        *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4 *>(to + C::kQTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    }
-                    now = next;
-                }
+    if (begin >= end) {  // nothing to do
+    } else if (warp < kSoftmaxWarps) {
+        // ================= softmax and results =================
+        const uint32_t lanes = (uint32_t)warp << 21;  // this warp's quarter of the TMEM lanes
+        const int row = threadIdx.x;
+        int count = 0;  // tiles so far
+        for (int k = 0;; ++k) {
+            const Segment &g = segment(k);
+            if (!ok || g.n == 0) break;
+            const int rows = g.rows, n = g.n, j0 = g.j0, len = g.s.len;
+            const bool live = row < rows, warp_live = warp * 32 < rows;
+            const int node = live ? (g.row0 + row) / p.t.group : 0;
+            uint32_t own0 = 0, own1 = 0;  // first mask bits
+            if (p.t.mask && live) {
+                const uint32_t *bits = p.t.mask + (int64_t)(g.s.first + node) * p.t.mask_words;
+                own0 = bits[0];
+                if (p.t.mask_words > 1) own1 = bits[1];
             }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_ready);
-
-            const int r = r_begin + (shared ? 0 : w * kSlotRows) + row;  // of the (sequence, KV head)
-            const bool live = r < r_begin + g.rows;
-            const int node = live ? r / p.t.group : 0;
-            const int warp_rows = g.rows - (shared ? 0 : w * kSlotRows) - (warp & 3) * 32;  // of this warp's 32
             float m = -INFINITY, l = 0.f;
-            int mine = 0;  // tiles of this slot in this segment
-            for (int i = shared ? w : 0; i < n; i += shared ? 2 : 1, ++mine, ++count) {
-                if (!mbar_wait_warp(s_full(w), count & 1, abort_flag)) {
-                    if (lane == 0) record_timeout(p, 300 + w);
+            for (int i = 0; i < n; ++i, ++count) {
+                const int b = count & 1;
+                if (!mbar_wait_warp(s_full(b), (count >> 1) & 1, abort_flag)) {
+                    if (lane == 0) record_timeout(p, 300 + b);
                     ok = false;
                     break;
                 }
-                if (warp_rows > 0) {
+                if (warp_live) {
                     tc_fence_after();
-                    const int t0 = (g.j0 + i) * kTok;
-                    const uint32_t valid = valid_s[(tile_base + i) % kValidRing];
-                    const bool masked = t0 + kTok > g.s.len || valid != 0xff;
-                    uint64_t on0 = ~0ull, on1 = ~0ull;
+                    uint32_t x[kTok];
+                    tmem_ld32(tmem_base + lanes + col_s(b), x);
+                    tmem_ld32(tmem_base + lanes + col_s(b) + 32, x + 32);
+                    const uint32_t valid = *reinterpret_cast<volatile uint8_t *>(&ctl.valid[count % kValidRing]);  // 16-token groups whose page is in the pool
+                    const int t0 = (j0 + i) * kTok;
+                    const bool masked = t0 + kTok > len || valid != 0xf;
+                    uint64_t on = ~0ull;
                     if (masked) {
-                        on0 = visible(p.t, g.s, node, t0, valid & 0xf);
-                        on1 = visible(p.t, g.s, node, t0 + 64, valid >> 4);
+                        on = visible(p.t, g.s, node, t0, own0 | (uint64_t)own1 << 32);
+                        for (int e = 0; e < 4; ++e)
+                            if (!((valid >> e) & 1)) on &= ~(0xffffull << (16 * e));
                     }
-                    // Scores 0..63 stay in registers from the maximum on, 64..127 are read again: P lies over the first half.
-                    uint32_t a[32], b[32];
-                    auto request = [&](int c, uint32_t (&x)[32]) { tmem_ld32(tmem_base + lanes + col_s(w) + 32 * c, x); };
-                    auto mask = [&](int c, uint32_t (&x)[32]) {
-                        if (!masked) return;
-                        const uint32_t bits = (uint32_t)((c & 2 ? on1 : on0) >> (32 * (c & 1)));
+                    tc_wait_ld();
+                    if (masked) {
+                        const uint32_t on0 = (uint32_t)on, on1 = (uint32_t)(on >> 32);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!((bits >> e) & 1)) x[e] = 0xff800000u;  // -inf
-                    };
+                        for (int e = 0; e < 32; ++e) {
+                            if (!((on0 >> e) & 1)) x[e] = 0xff800000u;  // -inf
+                            if (!((on1 >> e) & 1)) x[32 + e] = 0xff800000u;
+                        }
+                    }
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    auto maximum = [&](const uint32_t (&x)[32]) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(x[e]));
-                    };
-                    request(2, a);
-                    request(3, b);
-                    tc_wait_ld();
-                    mask(2, a);
-                    mask(3, b);
-                    maximum(a);
-                    maximum(b);
-                    request(0, a);
-                    request(1, b);
-                    tc_wait_ld();
-                    mask(0, a);
-                    mask(1, b);
-                    maximum(a);
-                    maximum(b);
+                    for (int e = 0; e < kTok; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(x[e]));
                     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    const bool grows = live && top > m + (mine ? kRescaleThreshold : 0.f);
+                    const bool grows = live && top > m + (i ? kRescaleThreshold : 0.f);
                     if (__any_sync(0xffffffffu, grows)) {
                         const float now = grows ? top : m, f = grows ? ex2(m - now) : 1.f;  // m = -inf gives 0
                         m = now;
                         l *= f;
-                        if (mine > 0) {
+                        if (i > 0) {  // the accumulator, which the value product before this tile still writes
+                            if (!mbar_wait_warp(pv_done(b ^ 1), ((count - 1) >> 1) & 1, abort_flag)) {
+                                if (lane == 0) record_timeout(p, 310 + b);
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
 #pragma unroll 1
                             for (int c = 0; c < D; c += 16) {
                                 uint32_t o[16];
-                                tmem_ld16(tmem_base + lanes + col_o(w) + c, o);
+                                tmem_ld16(tmem_base + lanes + c, o);
                                 tc_wait_ld();
 #pragma unroll
                                 for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                                tmem_st16(tmem_base + lanes + col_o(w) + c, o);
+                                tmem_st16(tmem_base + lanes + c, o);
                             }
                         }
                     }
                     const float base = m == -INFINITY ? 0.f : m;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                    auto weights = [&](int c, uint32_t (&x)[32]) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
-                            const float pa = ex2(__uint_as_float(x[e]) - base), pb = ex2(__uint_as_float(x[e + 1]) - base);
+                            const float pa = ex2(__uint_as_float(x[32 * h + e]) - base), pb = ex2(__uint_as_float(x[32 * h + e + 1]) - base);
                             sum[(e >> 1) & 3] += pa + pb;
-                            x[e / 2] = pack_bf16(pa, pb);
+                            x[32 * h + e / 2] = pack_bf16(pa, pb);
                         }
-                        tmem_st16(tmem_base + lanes + col_s(w) + 16 * c, x);
-                    };
-                    weights(0, a);
-                    request(2, a);
-                    weights(1, b);
-                    tc_wait_ld();
-                    request(3, b);
-                    mask(2, a);
-                    weights(2, a);
-                    tc_wait_ld();
-                    mask(3, b);
-                    weights(3, b);
+                        tmem_st16(tmem_base + lanes + col_s(b) + 16 * h, x + 32 * h);
+                    }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     tc_wait_st();
                     tc_fence_before();
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full(w));
+                if (lane == 0) mbar_arrive(p_full(b));
             }
-            tile_base += n;
             if (!ok) break;
-            if (mine > 0) {
-                if (!mbar_wait_warp(o_final(w), finals++ & 1, abort_flag)) {
-                    if (lane == 0) record_timeout(p, 320 + w);
+            // ---- results, while the next segment's first scores are formed
+            if (!mbar_wait_warp(pv_done((count - 1) & 1), ((count - 1) >> 1) & 1, abort_flag)) {
+                if (lane == 0) record_timeout(p, 320);
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            if (warp_live) {
+                const bool whole = g.parts == 1, nothing = l == 0.f;
+                const int64_t part = (int64_t)blockIdx.x * 2 + (j0 == 0 ? 1 : 0);
+                const int64_t out = (int64_t)(g.s.first + node) * p.t.q_heads + g.kv_head * p.t.group + (live ? g.row0 + row - node * p.t.group : 0);
+                const float keep = nothing ? 0.f : whole ? 1.0f / l : 1.f;
+                const int poison = *reinterpret_cast<volatile uint8_t *>(&ctl.poison[k % kPoisonRing]);
+                if (live) {
+                    if (whole) p.t.lse[out] = nothing ? -INFINITY : (m + log2f(l)) * kLn2;
+                    else p.part_ml[part * ROWS + row] = make_float2(m, l);
+                }
+                uint4 *to = reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.t.o) + out * D);
+                float4 *to_part = p.part_o + part * (D / 4) * ROWS + row;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 16) {
+                    uint32_t raw[16];
+                    float o[16];
+                    tmem_ld16(tmem_base + lanes + c, raw);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] = nothing ? 0.f : __uint_as_float(raw[e]) * keep;
+                    if (!live) continue;
+                    if (poison) add_not_finite(p.t, g.s, g.seq, g.kv_head, node, j0 * kTok, (j0 + n) * kTok, c, o);
+                    if (whole) {
+                        to[c / 8] = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
+                        to[c / 8 + 1] = make_uint4(pack_bf16(o[8], o[9]), pack_bf16(o[10], o[11]), pack_bf16(o[12], o[13]), pack_bf16(o[14], o[15]));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) to_part[(c / 4 + e) * ROWS] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    }
+                }
+            }
+            tc_fence_before();  // the next segment's first value product starts the accumulator anew, behind this warp's next P
+            if (g.parts > 1) {
+                __syncwarp();
+                if (lane == 0) {
+                    __threadfence();
+                    if (atomicInc(&p.arrived[g.cta], kSoftmaxWarps * g.parts - 1) == kSoftmaxWarps * g.parts - 1u) {  // the last one's CTA joins
+                        __threadfence();
+                        ctl.join[j0 > 0 && !(j0 + n < g.tiles) ? 0 : 1] = Join{g.s.first, g.kv_head, g.row0, rows, g.parts, g.cta};
+                    }
+                }
+            }
+        }
+    } else if (warp < kQWarp + kQWarps) {
+        // ================= planning; queries =================
+        // A segment is planned once the queries of the one two before it are not needed any more.  By then its last scores have been
+        // asked for, and with them the value products of the segment before: no warp has to do with anything before that one, which is three
+        // before the planned one, and the ring holds four.
+        // (The way along the span and what is planned next lie in shared memory: there is no room for them beside the queries.)
+        const bool plans = warp == kQWarp;
+        bool more = plans;  // the end is not planned yet
+        auto plan = [&]() {
+            Walk<ROWS> walk = ctl.walk;
+            Segment coming;
+            walk.next(p, coming);
+            __syncwarp();
+            if (lane == 0) {
+                ctl.walk = walk;
+                ctl.coming = coming;
+            }
+            __syncwarp();
+        };
+        auto publish = [&](int k) {
+            more = ctl.coming.n > 0;
+            __syncwarp();
+            if (lane == 0) {
+                ctl.seg[k % kSegRing] = ctl.coming;
+                mbar_arrive(planned(k));
+            }
+            __syncwarp();
+        };
+        if (plans) {
+            const Walk<ROWS> walk{begin, end, ctl.start.seq_start, ctl.start.units, span, ctl.start.seq, ctl.start.s};
+            __syncwarp();
+            if (lane == 0) ctl.walk = walk;
+            __syncwarp();
+#pragma unroll 1
+            for (int k = 0; k < 2 && more; ++k) {
+                plan();
+                publish(k);
+            }
+        }
+        const int tid = threadIdx.x - kQWarp * 32, quads = (p.t.group + 3) / 4;
+        static_assert(kQWarps * 32 % (D / 8) == 0, "a thread's dims");
+        const int c = tid % (D / 8);  // its 8 dims, of whatever token
+        uint64_t turns[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) turns[e] = p.t.freq.turns[c * 4 + e];
+        for (int k = 0;; ++k) {
+            const Segment &g = segment(k);
+            if (!ok || g.n == 0) break;
+            const int node0 = g.row0 / p.t.group, nodes = (g.row0 + g.rows - 1) / p.t.group + 1 - node0, row0 = g.row0 - node0 * p.t.group, rows = g.rows;
+            const int tasks = nodes * quads * (D / 8), head0 = g.kv_head * p.t.group, first = g.s.first + node0;
+            // A thread takes 8 dims of up to four heads of a drafted token, whose angles are the same, kQSteps tokens' at a time: all
+            // loads of 64 rows (of groups of four) are in flight while the last scores of the segment before are formed.
+            uint4 raw[kQSteps][4];
+            int position[kQSteps];
+            auto request = [&](int base) {
+#pragma unroll
+                for (int u = 0; u < kQSteps; ++u) {
+                    const int i = base + u * kQWarps * 32;
+                    if (i >= tasks) break;
+                    const int nq = i / (D / 8), node = quads == 1 ? nq : nq / quads, h = (nq - node * quads) * 4;
+                    position[u] = p.t.positions[first + node];
+                    const char *from = static_cast<const char *>(p.t.q) + (((int64_t)(first + node) * p.t.q_heads + head0 + h) * D + c * 8) * 2;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (h + e < p.t.group && (unsigned)(node * p.t.group + h + e - row0) < (unsigned)rows) raw[u][e] = *reinterpret_cast<const uint4 *>(from + e * D * 2);
+                }
+            };
+            const bool planning = k > 0 && more;
+            if (planning) plan();
+            request(tid);
+            if (k > 0) {
+                if (!mbar_wait_warp(q_empty, (k - 1) & 1, abort_flag)) {
+                    if (lane == 0) record_timeout(p, 330);
                     ok = false;
                     break;
                 }
-                tc_fence_after();
-            }
-            // where this warp's rows pass on their way out: over the queries, which no product reads any more (of the shared ones, once
-            // both slots are through)
-            uint8_t *stage = q_s + (shared ? 0 : w * 2 * C::kQTile) + (warp & 3) * (32 * D * 4);
-            // ---- the slots' states, where they share rows, are joined by slot 0, which reads both accumulators
-            float keep = 1.f, other = 0.f;  // factors of this slot's accumulator and of slot 1's
-            if (shared) {
-                float2 *join_ml = reinterpret_cast<float2 *>(stage);
-                if (w == 1) {
-                    if (mine > 0) join_ml[lane] = make_float2(m, l);
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(join_full);
-                } else {
-                    if (!mbar_wait_warp(join_full, joins++ & 1, abort_flag)) {
-                        if (lane == 0) record_timeout(p, 340);
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    if (n > 1) {
-                        const float2 ml = join_ml[lane];
-                        const float mx = fmaxf(m, ml.x);
-                        keep = l == 0.f ? 0.f : ex2(m - mx);  // a slot that has seen nothing counts for nothing; a NaN counts
-                        other = ml.y == 0.f ? 0.f : ex2(ml.x - mx);
-                        l = (l == 0.f ? 0.f : keep * l) + (ml.y == 0.f ? 0.f : other * ml.y);
-                        m = mx;
-                        __syncwarp();
-                    }
-                }
-            }
-            const bool whole = g.j0 == 0 && g.j1 == g.tiles;
-            if (warp_rows > 0 && !(shared && w == 1)) {
-                const int64_t part = ((int64_t)blockIdx.x * 2 + (g.j0 == 0 ? 1 : 0)) * kItemRows + (r - r_begin);
-                const int64_t out = (int64_t)(g.s.first + node) * p.t.q_heads + g.kv_head * p.t.group + (live ? r % p.t.group : 0);
-                const bool nothing = l == 0.f;
-                const float inv = whole ? (nothing ? 0.f : 1.0f / l) : 1.f;
-                keep *= inv;
-                other *= inv;
-                const int poison = *reinterpret_cast<volatile int *>(&poison_s[k % kPoisonRing]);
-#pragma unroll 1
-                for (int c = 0; c < D; c += 16) {
-                    uint32_t raw[16], raw1[16];
-                    float o[16];
-                    tmem_ld16(tmem_base + lanes + col_o(w) + c, raw);
-                    if (shared && n > 1) tmem_ld16(tmem_base + lanes + col_o(1) + c, raw1);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        o[e] = keep == 0.f ? 0.f : __uint_as_float(raw[e]) * keep;
-                        if (shared && n > 1 && other != 0.f) o[e] = fmaf(__uint_as_float(raw1[e]), other, o[e]);
-                    }
-                    if (poison && live) {  // drafted tokens of this segment whose V is not finite, for the rows that see them
-                        for (int t = max(g.s.len, g.j0 * kTok); t < min(g.s.tokens, g.j1 * kTok); ++t) {
-                            if (!tree_sees(p.t, g.s, node, t - g.s.len)) continue;
-                            const int page = p.t.page_tables[(int64_t)g.seq * p.t.max_pages + t / p.t.page_size];
-                            if ((unsigned)page >= (unsigned)p.t.physical_pages) continue;
-                            const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(p.t.v) +
-                                                     (((int64_t)page * p.t.page_size + t % p.t.page_size) * p.t.kv_heads + g.kv_head) * D + c;
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const float y = __bfloat162float(v[e]);
-                                if (!isfinite(y)) o[e] += y;
-                            }
-                        }
-                    }
-                    // 16-byte chunks of a row, exchanged within groups of eight so that neither side meets a bank twice
-                    if (whole) {
-                        uint8_t *to = stage + lane * (D * 2);
-                        *reinterpret_cast<uint4 *>(to + (((c / 8) ^ (lane & 7)) << 4)) =
-                            make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
-                        *reinterpret_cast<uint4 *>(to + (((c / 8 + 1) ^ (lane & 7)) << 4)) =
-                            make_uint4(pack_bf16(o[8], o[9]), pack_bf16(o[10], o[11]), pack_bf16(o[12], o[13]), pack_bf16(o[14], o[15]));
-                    } else {
-                        uint8_t *to = stage + lane * (D * 4);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            *reinterpret_cast<float4 *>(to + (((c / 4 + e) ^ (lane & 7)) << 4)) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                    }
-                }
-                if (live) {
-                    if (whole) p.t.lse[out] = nothing ? -INFINITY : (m + log2f(l)) * kLn2;
-                    else p.part_ml[part] = make_float2(m, l);
-                }
+                if (planning) publish(k + 1);
+            } else {
+                // The ring's first filling is 24 MB of the whole device: the first queries would arrive behind it, 7000 clk later.
+                uint32_t seen = 0;
+                if (tid < tasks) asm volatile("mov.b32 %0, %1;" : "=r"(seen) : "r"(raw[0][0].x));
                 __syncwarp();
-                const int rows = min(32, warp_rows);
-                if (whole) {
-                    constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;  // lanes of a row
-                    const int c = lane % kLanes;
-#pragma unroll 4
-                    for (int i = 0; i < 32; i += kAtOnce) {
-                        const int rr = i + lane / kLanes;
-                        const int64_t to = __shfl_sync(0xffffffffu, out, rr);
-                        if (rr < rows)
-                            reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.t.o) + to * D)[c] =
-                                *reinterpret_cast<const uint4 *>(stage + rr * (D * 2) + ((c ^ (rr & 7)) << 4));
-                    }
+                if (lane == 0) mbar_arrive(go);
+            }
+#pragma unroll 1
+            for (int i = tid, step = 0; i < tasks; i += kQWarps * 32) {
+                const int nq = i / (D / 8), node = quads == 1 ? nq : nq / quads, h = (nq - node * quads) * 4;
+                float2 cs[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    cs[e] = turn_of_fast(position[0], turns[e]);
+                    cs[e].x *= p.t.scale * kLog2e;
+                    cs[e].y *= p.t.scale * kLog2e;
+                }
+#pragma unroll 1
+                for (int r = node * p.t.group + h - row0, e = h; e < min(h + 4, p.t.group); ++e, ++r) {
+                    if ((unsigned)r < (unsigned)rows) write_query<C::kQTile>(raw[0][0], cs, q_s + (c >> 3) * C::kQBox + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                    raw[0][0] = raw[0][1], raw[0][1] = raw[0][2], raw[0][2] = raw[0][3];  // registers move so that the loops stay loops
+                }
+                if (++step == kQSteps) {
+                    step = 0;
+                    request(i + kQWarps * 32);
                 } else {
-                    constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;
-                    const int c = lane % kLanes;
-                    const int64_t first = __shfl_sync(0xffffffffu, part, 0);
-#pragma unroll 4
-                    for (int i = 0; i < 32; i += kAtOnce) {
-                        const int rr = i + lane / kLanes;
-                        if (rr < rows)
-                            reinterpret_cast<uint4 *>(p.part_o + (first + rr) * D)[c] =
-                                *reinterpret_cast<const uint4 *>(stage + rr * (D * 4) + ((c ^ (rr & 7)) << 4));
+#pragma unroll
+                    for (int u = 0; u + 1 < kQSteps; ++u) {
+                        position[u] = position[u + 1];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) raw[u][e] = raw[u + 1][e];
                     }
                 }
             }
-            tc_fence_before();  // the next segment's first value product starts the accumulator anew
-            if (threadIdx.x == 0 && g.j0 == 0 && !whole) {
-                Record &to = p.records[blockIdx.x];
-                to.seq = g.seq;
-                to.kv_head = g.kv_head;
-                to.pair = g.pair;
-                to.parts = (int)((g.item_end - 1) / span) - (int)blockIdx.x + 1;
-            }
+            fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(q_free);
+            if (lane == 0) mbar_arrive(q_ready);
         }
     } else if (warp == kKWarp || warp == kVWarp) {
         // ================= TMA producers: K tiles and V tiles =================
@@ -660,28 +602,33 @@ template <int D, bool NARROW> __global__ void __launch_bounds__(kThreads, 1) tre
         const int boxes = kTok / p.box_rows, groups = p.box_rows / 8, page_groups = p.t.page_size / 8;
         const int no_group = p.t.physical_pages * page_groups;  // behind the pool: zeros
         uint32_t order = 0;  // tiles of the ring before the segment
-        int tile_base = 0;
-        bool ok = true;
-        while (ok && walk.next(p.t, g)) {
-            const int n = g.j1 - g.j0, ahead = NARROW || g.rows <= kSlotRows ? 2 : 1;
+        int count = 0;
+        for (int k = 0;; ++k) {
+            const Segment g = segment(k);
+            if (!ok || g.n == 0) break;
             BoxRows rows;
-            rows.start(p.t, g, p.box_rows);
-            for (int i = 0; ok && i < n; ++i) {
+            rows.start(p.t, g.seq, g.s.tokens, g.j0 * kTok, p.box_rows);
+            if (k == 0 && !mbar_wait_warp(go, 0, abort_flag)) {
+                if (lane == 0) record_timeout(p, 110);
+                ok = false;
+                break;
+            }
+            for (int i = 0; i < g.n; ++i, ++count) {
                 const int first = (g.j0 + i) * boxes;
                 rows.seek(first);
                 const bool bad = rows.page == -1 || rows.page >= p.t.physical_pages;
                 const int group = rows.page < 0 || bad ? no_group : rows.page * page_groups + (rows.in_page >> 3);
                 if (is_k) {
-                    uint32_t valid = 0xff;
+                    uint32_t valid = 0xf;
                     const uint32_t all = __ballot_sync(0xffffffffu, bad) >> (first - rows.base);
                     if (all) {
-                        for (int e = 0; e < 8; ++e)
+                        for (int e = 0; e < 4; ++e)
                             if ((all >> (e * 16 / p.box_rows)) & 1 && e * 16 / p.box_rows < boxes) valid &= ~(1u << e);
-                        if (lane == 0 && valid != 0xff) tree_report(p.t, FLAT_ERR_PAGE_OUT_OF_RANGE, g.seq);
+                        if (lane == 0 && valid != 0xf) tree_report(p.t, FLAT_ERR_PAGE_OUT_OF_RANGE, g.seq);
                     }
-                    if (lane == 0) valid_s[(tile_base + i) % kValidRing] = valid;
+                    if (lane == 0) ctl.valid[count % kValidRing] = (uint8_t)valid;
                 }
-                const uint32_t at = order + (is_k ? k_entry(i, ahead) : v_entry(i, n, ahead));
+                const uint32_t at = order + (is_k ? k_entry(i, kAhead) : v_entry(i, g.n, kAhead));
                 const int s = at % C::kStages;
                 if (!mbar_wait_warp(empty(s), ((at / C::kStages) & 1) ^ 1, abort_flag)) {
                     if (lane == 0) record_timeout(p, 100 + s);
@@ -698,8 +645,8 @@ template <int D, bool NARROW> __global__ void __launch_bounds__(kThreads, 1) tre
                 }
                 if (!is_k && leader && is_tail(g, g.j0 + i)) mbar_arrive(to_fix(s));
             }
-            order += 2 * n;
-            tile_base += n;
+            if (!ok) break;
+            order += 2 * g.n;
         }
     } else if (warp == kMmaWarp) {
         // ================= all products =================
@@ -709,8 +656,7 @@ template <int D, bool NARROW> __global__ void __launch_bounds__(kThreads, 1) tre
             const uint32_t v_desc = (uint32_t)make_smem_desc(smem_u32(kv_s), 1024, C::kGroup);
             constexpr uint32_t kTile16 = C::kKvTile >> 4;
             uint32_t order = 0, fixed_phase = 0;
-            int valued[2] = {0, 0};  // tiles per slot
-            bool ok = true;
+            int done = 0;  // tiles of the segments before
             auto wait = [&](uint32_t bar, uint32_t parity, int where) {
                 if (ok && !mbar_wait(bar, parity, abort_flag)) {
                     record_timeout(p, where);
@@ -722,101 +668,63 @@ template <int D, bool NARROW> __global__ void __launch_bounds__(kThreads, 1) tre
                 wait(full(at % C::kStages), (at / C::kStages) & 1, 210);
                 return (int)(at % C::kStages);
             };
-            auto scores = [&](int w, int q_slot, int s) {
+            auto scores = [&](int i, int n) {
+                const int b = (done + i) & 1, s = landed(k_entry(i, kAhead));
                 if (!ok) return;
                 tc_fence_after();
-                const uint32_t q = q_desc + q_slot * (2 * C::kQTile >> 4), kk = k_desc + s * kTile16, d = tmem_base + col_s(w);
+                const uint32_t kk = k_desc + s * kTile16, d = tmem_base + col_s(b);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)  // the two summands of q
 #pragma unroll
                     for (int e = 0; e < D / 16; ++e)
-                        mma_scores<C::kGroup>(d, q + h * (C::kQTile >> 4) + (e >> 2) * (C::kQBox >> 4) + (e & 3) * 2,
+                        mma_scores<C::kGroup>(d, q_desc + h * (C::kQTile >> 4) + (e >> 2) * (C::kQBox >> 4) + (e & 3) * 2,
                                               kk + (e >> 2) * (1024 >> 4) + (e & 3) * 2, p.idesc_qk, h > 0 || e > 0);
-                tc_commit(s_full(w));
+                tc_commit(s_full(b));
+                tc_commit(empty(s));
+                if (i + 1 == n) tc_commit(q_empty);
             };
-            auto values = [&](int w, int s, bool first, bool last) {
-                wait(p_full(w), valued[w]++ & 1, 240 + w);
+            auto values = [&](int v, const Segment &g) {
+                const int b = (done + v) & 1, s = landed(v_entry(v, g.n, kAhead));
+                if (is_tail(g, g.j0 + v)) {
+                    wait(fixed(s), (fixed_phase >> s) & 1, 230);
+                    fixed_phase ^= 1u << s;
+                }
+                wait(p_full(b), ((done + v) >> 1) & 1, 240 + b);
                 if (!ok) return;
                 tc_fence_after();
 #pragma unroll
                 for (int e = 0; e < kTok / 16; ++e)
-                    mma_values<C::kGroup>(tmem_base + col_o(w), tmem_base + col_s(w) + e * 8, v_desc + s * kTile16 + e * (2 * C::kGroup >> 4), p.idesc_pv,
-                                          !first || e > 0);
-                if (last) tc_commit(o_final(w));
+                    mma_values<C::kGroup>(tmem_base, tmem_base + col_s(b) + e * 8, v_desc + s * kTile16 + e * (2 * C::kGroup >> 4), p.idesc_pv, v > 0 || e > 0);
+                tc_commit(pv_done(b));
+                tc_commit(empty(s));
             };
-            auto fixed_tile = [&](int v, int s) {
-                if (!is_tail(g, g.j0 + v)) return;
-                wait(fixed(s), (fixed_phase >> s) & 1, 230);
-                fixed_phase ^= 1u << s;
-            };
-            for (int k = 0; ok && walk.next(p.t, g); ++k) {
-                const int n = g.j1 - g.j0;
+            for (int k = 0;; ++k) {
+                wait(planned(k), (k / kSegRing) & 1, 506);
+                if (!ok) break;
+                const Segment g = ctl.seg[k % kSegRing];
+                if (g.n == 0) break;
                 wait(q_ready, k & 1, 200);
-                if (NARROW || g.rows <= kSlotRows) {
-                    for (int i = 0; i < min(n, 2); ++i) {
-                        const int s = landed(k_entry(i, 2));
-                        scores(i, 0, s);
-                        if (ok) tc_commit(empty(s));
-                    }
-                    for (int v = 0; ok && v < n; ++v) {
-                        const int w = v & 1, s = landed(v_entry(v, n, 2));
-                        fixed_tile(v, s);
-                        values(w, s, v < 2, v + 2 >= n);
-                        if (ok) tc_commit(empty(s));
-                        if (v + 2 < n) {
-                            const int sk = landed(k_entry(v + 2, 2));
-                            scores(w, 0, sk);
-                            if (ok) tc_commit(empty(sk));
-                        }
-                    }
-                } else {
-                    int sk = landed(0);
-                    scores(0, 0, sk);
-                    scores(1, 1, sk);
-                    if (ok) tc_commit(empty(sk));
-                    for (int v = 0; ok && v < n; ++v) {
-                        const int s = landed(v_entry(v, n, 1));
-                        fixed_tile(v, s);
-                        values(0, s, v == 0, v + 1 == n);
-                        if (v + 1 < n) {
-                            sk = landed(k_entry(v + 1, 1));
-                            scores(0, 0, sk);
-                        }
-                        values(1, s, v == 0, v + 1 == n);
-                        if (ok) tc_commit(empty(s));
-                        if (v + 1 < n) {
-                            scores(1, 1, sk);
-                            if (ok) tc_commit(empty(sk));
-                        }
-                    }
+#pragma unroll 1
+                for (int i = 0; ok && i < g.n + kAhead; ++i) {
+                    if (i >= kAhead) values(i - kAhead, g);
+                    if (i < g.n) scores(i, g.n);
                 }
-                order += 2 * n;
+                if (!ok) break;
+                done += g.n;
+                order += 2 * g.n;
             }
         }
     } else {
-        // ================= V tiles with drafted tokens or the end of a sequence; the next segment's queries into the L2 =================
+        // ================= V tiles with drafted tokens or the end of a sequence =================
         uint32_t order = 0, phase = 0;
-        bool ok = true;
-        Walk coming = walk;
-        Segment c;
-        bool more = coming.next(p.t, c);  // the first segment itself
-        for (int k = 0; ok && walk.next(p.t, g); ++k) {
-            const int n = g.j1 - g.j0, ahead = NARROW || g.rows <= kSlotRows ? 2 : 1;
-            if (lane == 0) poison_s[k % kPoisonRing] = 0;
+        for (int k = 0;; ++k) {
+            const Segment g = segment(k);
+            if (!ok || g.n == 0) break;
+            if (lane == 0) ctl.poison[k % kPoisonRing] = 0;
             __syncwarp();
-            more = more && coming.next(p.t, c);
-            if (more) {
-                const int r0 = c.pair * kItemRows;
-                for (int i = lane; i < c.rows * C::kBoxes; i += 32) {  // 128 bytes each
-                    const int r = r0 + i / C::kBoxes;
-                    const char *at = static_cast<const char *>(p.t.q) +
-                                     ((int64_t)(c.s.first + r / p.t.group) * p.t.q_heads + c.kv_head * p.t.group + r % p.t.group) * (D * 2) + i % C::kBoxes * 128;
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
-                }
-            }
             // (to_fix tells that the tile before in this stage is used up, without which its phase could be taken for this one's)
-            for (int v = max(0, min(g.s.len / kTok, g.tiles - 1) - g.j0); v < n; ++v) {
-                const uint32_t at = order + v_entry(v, n, ahead);
+            for (int v = max(0, min(g.s.len / kTok, g.tiles - 1) - g.j0); v < g.n; ++v) {
+                const uint32_t at = order + v_entry(v, g.n, kAhead);
                 const int s = at % C::kStages;
                 if (!mbar_wait_warp(to_fix(s), (phase >> s) & 1, abort_flag) || !mbar_wait_warp(full(s), (at / C::kStages) & 1, abort_flag)) {
                     if (lane == 0) record_timeout(p, 400);
@@ -824,38 +732,15 @@ template <int D, bool NARROW> __global__ void __launch_bounds__(kThreads, 1) tre
                     break;
                 }
                 phase ^= 1u << s;
-                const int t0 = (g.j0 + v) * kTok, from = max(0, min(g.s.len, g.s.tokens) - t0), live = g.s.tokens - t0;
-                uint8_t *tile = kv_s + s * C::kKvTile;
-                bool met = false;
-#pragma unroll 2
-                for (int i = lane; i < (kTok - from) * C::kBoxes * 8; i += 32) {
-                    const int row = from + i / (C::kBoxes * 8), e8 = i % (C::kBoxes * 8);
-                    uint4 *x = reinterpret_cast<uint4 *>(tile + (row >> 3) * C::kGroup + (e8 >> 3) * 1024 + (row & 7) * 128 + ((e8 & 7) << 4));
-                    if (row >= live) {
-                        *x = make_uint4(0, 0, 0, 0);
-                        continue;
-                    }
-                    const uint4 y = *x;
-                    const uint32_t in[4] = {y.x, y.y, y.z, y.w};
-                    uint32_t out[4];
-                    bool bad = false;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        out[e] = in[e];
-                        if ((in[e] & 0x7f80u) == 0x7f80u) out[e] &= 0xffff0000u, bad = true;
-                        if ((in[e] & 0x7f800000u) == 0x7f800000u) out[e] &= 0x0000ffffu, bad = true;
-                    }
-                    if (bad) {
-                        *x = make_uint4(out[0], out[1], out[2], out[3]);
-                        met = true;
-                    }
-                }
-                if (__any_sync(0xffffffffu, met) && lane == 0) poison_s[k % kPoisonRing] = 1;
+                const int t0 = (g.j0 + v) * kTok;
+                const bool met = clear_values<C::kBoxes, kTok>(kv_s + s * C::kKvTile, max(0, min(g.s.len, g.s.tokens) - t0), g.s.tokens - t0);
+                if (__any_sync(0xffffffffu, met) && lane == 0) ctl.poison[k % kPoisonRing] = 1;
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(fixed(s));
             }
-            order += 2 * n;
+            if (!ok) break;
+            order += 2 * g.n;
         }
     }
 
@@ -866,98 +751,39 @@ template <int D, bool NARROW> __global__ void __launch_bounds__(kThreads, 1) tre
     __syncthreads();
     if (warp == kMmaWarp) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, 512);
+        tmem_dealloc(tmem_base, 512 / kCtasPerSm);
     }
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i)
+        if (ctl.join[i].parts) join_parts<D, ROWS>(p, ctl.join[i]);
 }
 
-// Joins the parts of an item that begins in CTA blockIdx.x and ends in a later one, in CTA order: 32 rows a block, a row a warp.
-template <int D> __global__ void __launch_bounds__(256) tree_sm100_merge_kernel(const __grid_constant__ KernelParams p) {
-    grid_dependency_wait();
-    grid_dependency_launch();
-    const Record rec = p.records[blockIdx.x];
-    if (rec.parts <= 0) return;
-    const TreeSequence s = tree_sequence(p.t, rec.seq);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r_begin = rec.pair * kItemRows;
-    const int rows = min(kItemRows, s.nodes * p.t.group - r_begin);
-    constexpr int kPer = D / 32;
-    for (int r = blockIdx.y * 32 + warp; r < min(rows, (int)blockIdx.y * 32 + 32); r += 8) {
-        auto slot = [&](int i) { return (int64_t)((blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kItemRows + r; };
-        float mx = -INFINITY;
-        for (int i = lane; i < rec.parts; i += 32) mx = fmaxf(mx, p.part_ml[slot(i)].x);
-#pragma unroll
-        for (int d = 16; d >= 1; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-        float sum = 0.f, o[kPer] = {};
-#pragma unroll 4
-        for (int i = 0; i < rec.parts; ++i) {
-            const float2 ml = p.part_ml[slot(i)];
-            const float *from = p.part_o + slot(i) * D + lane * kPer;
-            float x[kPer];
-            if constexpr (kPer == 4) {
-                const float4 y = *reinterpret_cast<const float4 *>(from);
-                x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
-            } else {
-                const float2 y = *reinterpret_cast<const float2 *>(from);
-                x[0] = y.x, x[1] = y.y;
-            }
-            if (ml.y == 0.f) continue;  // a part in which the row has seen nothing; a NaN counts
-            const float f = ex2(ml.x - mx);
-            sum = fmaf(f, ml.y, sum);
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) o[e] = fmaf(f, x[e], o[e]);
-        }
-        const bool nothing = sum == 0.f;
-        const float inv = nothing ? 0.f : 1.0f / sum;
-        const int row = r_begin + r;
-        const int64_t out = (int64_t)(s.first + row / p.t.group) * p.t.q_heads + rec.kv_head * p.t.group + row % p.t.group;
-        uint32_t *to = reinterpret_cast<uint32_t *>(static_cast<__nv_bfloat16 *>(p.t.o) + out * D + lane * kPer);
-#pragma unroll
-        for (int e = 0; e < kPer; e += 2) to[e / 2] = pack_bf16(o[e] * inv, o[e + 1] * inv);
-        if (lane == 0) p.t.lse[out] = nothing ? -INFINITY : (mx + log2f(sum)) * kLn2;
-    }
-}
-
-// 5-D map over (64 dims, token of 8, 64-dim block, group of 8 tokens, head) of a pool, with a box of one head's `box_rows` tokens.
-int make_pool_map(flat_ctx *ctx, CUtensorMap *map, const void *base, int head_dim, uint64_t rows, int kv_heads, int box_rows) {
-    EncodeFn fn = encode_fn();
-    if (!fn) return fail(ctx, FLAT_ERR_UNAVAILABLE, "cuTensorMapEncodeTiled is not available from this driver");
-    const cuuint64_t row_bytes = (cuuint64_t)kv_heads * head_dim * 2;
-    cuuint64_t dims[5] = {64, 8, (cuuint64_t)head_dim / 64, rows / 8, (cuuint64_t)kv_heads};
-    cuuint64_t strides[4] = {row_bytes, 128, row_bytes * 8, (cuuint64_t)head_dim * 2};
-    cuuint32_t box[5] = {64, 8, (cuuint32_t)head_dim / 64, (cuuint32_t)box_rows / 8, 1};
-    cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(ctx, FLAT_ERR_EXECUTION, "cuTensorMapEncodeTiled failed with %d", (int)r);
-    return FLAT_OK;
-}
-
-template <int D, bool NARROW> int launch(flat_ctx *ctx, const TreeParams &t) {
-    using C = Cfg<D, NARROW>;
+template <int D, int ROWS> int launch(flat_ctx *ctx, const TreeParams &t) {
+    using C = Cfg<D, ROWS>;
     KernelParams p{};
     p.t = t;
-    p.box_rows = t.page_size % 128 == 0 ? 128 : t.page_size % 64 == 0 ? 64 : t.page_size % 32 == 0 ? 32 : 16;
+    p.share = (int64_t)t.max_nodes * t.group > ROWS ? 2 : 1;
+    p.box_rows = t.page_size % 64 == 0 ? 64 : t.page_size % 32 == 0 ? 32 : 16;
     const uint64_t rows = (uint64_t)t.physical_pages * t.page_size;
     if (int st = make_pool_map(ctx, &p.map_k, t.k, D, rows, t.kv_heads, p.box_rows)) return st;
     if (int st = make_pool_map(ctx, &p.map_v, t.v, D, rows, t.kv_heads, p.box_rows)) return st;
-    p.idesc_qk = make_idesc(kFmtBF16, kFmtBF16, 0, 0, kSlotRows, kTok);
-    p.idesc_pv = make_idesc(kFmtBF16, kFmtBF16, 0, 1, kSlotRows, D);
-    const int grid = ctx->sm_count;
+    p.idesc_qk = make_idesc(kFmtBF16, kFmtBF16, 0, 0, kMmaRows, kTok);
+    p.idesc_pv = make_idesc(kFmtBF16, kFmtBF16, 0, 1, kMmaRows, D);
+    const int grid = ctx->sm_count * kCtasPerSm;
+    static_assert(kCtasPerSm == 2, "the grid has to be even");
     char *at = static_cast<char *>(ctx->paged_scratch) + kPagedPlanBytes;
-    const uint64_t rows_held = (uint64_t)grid * 2 * kItemRows;
+    const uint64_t rows_held = (uint64_t)grid * 2 * ROWS;
     const uint64_t o_bytes = rows_held * D * sizeof(float), ml_bytes = rows_held * sizeof(float2);
-    if (o_bytes + ml_bytes + grid * sizeof(Record) > kPagedScratchBytes - kPagedPlanBytes)
+    if (o_bytes + ml_bytes > kPagedScratchBytes - kPagedPlanBytes || (uint64_t)grid > kPagedTickets)
         return fail(ctx, FLAT_ERR_EXECUTION, "the scratch does not hold the parts of %d CTAs", grid);
-    p.part_o = reinterpret_cast<float *>(at);
+    p.part_o = reinterpret_cast<float4 *>(at);
     p.part_ml = reinterpret_cast<float2 *>(at + o_bytes);
-    p.records = reinterpret_cast<Record *>(at + o_bytes + ml_bytes);
-    FLAT_CUDA_OK(ctx, cudaFuncSetAttribute(tree_sm100_kernel<D, NARROW>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    p.arrived = paged_tickets(ctx) + 1;
+    FLAT_CUDA_OK(ctx, cudaFuncSetAttribute(tree_sm100_kernel<D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     {
         KernelTimer timer(ctx);
-        FLAT_CUDA_OK(ctx, launch_dependent(may_overlap_previous(ctx), tree_sm100_kernel<D, NARROW>, dim3((unsigned)grid), kThreads, C::kSmem, ctx->stream, p));
+        FLAT_CUDA_OK(ctx, launch_dependent(may_overlap_previous(ctx), tree_sm100_kernel<D, ROWS>, dim3((unsigned)grid), C::kThreads, C::kSmem, ctx->stream, p));
     }
-    ctx->launches += 1;
-    const int chunks = (int)std::min<int64_t>(kMergeChunks, ((int64_t)t.max_nodes * t.group + 31) / 32);
-    FLAT_CUDA_OK(ctx, launch_dependent(true, tree_sm100_merge_kernel<D>, dim3((unsigned)grid, (unsigned)chunks), 256, 0, ctx->stream, p));
     ctx->launches += 1;
     return FLAT_OK;
 }
@@ -965,14 +791,16 @@ template <int D, bool NARROW> int launch(flat_ctx *ctx, const TreeParams &t) {
 }  // namespace
 
 bool tree_sm100_supported(int dtype, const TreeParams &p) {
+    // the line's length is a 32-bit number
+    const int64_t blocks = ((int64_t)p.max_nodes * p.group + 63) / 64, tiles = (std::min<int64_t>(p.max_context, (int64_t)p.max_pages * p.page_size) + kTok - 1) / kTok;
     return dtype == FLAT_BF16 && (p.head_dim == 64 || p.head_dim == 128) && p.page_size % 16 == 0 &&
-           ((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.o) % 16 == 0;
+           ((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.o) % 16 == 0 && blocks * p.kv_heads * p.num_seqs < (1ll << 30) / tiles;
 }
 
 int launch_tree_sm100(flat_ctx *ctx, const TreeParams &p) {
-    const bool narrow = (int64_t)p.max_nodes * p.group <= kSlotRows;
-    if (p.head_dim == 128) return narrow ? launch<128, true>(ctx, p) : launch<128, false>(ctx, p);
-    return narrow ? launch<64, true>(ctx, p) : launch<64, false>(ctx, p);
+    const bool few = (int64_t)p.max_nodes * p.group <= 64;
+    if (p.head_dim == 128) return few ? launch<128, 64>(ctx, p) : launch<128, 128>(ctx, p);
+    return few ? launch<64, 64>(ctx, p) : launch<64, 128>(ctx, p);
 }
 
 }  // namespace flat
