@@ -51,7 +51,8 @@ __device__ __forceinline__ bool sees(const TreeParams &p, const TreeSequence &s,
     return token < s.len || (token - s.len < s.nodes && tree_sees(p, s, node, token - s.len));
 }
 
-template <typename T> __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_constant__ TreeParams p) {
+// HALVES: of 64 dims (head_dim up to 64 or 128).
+template <typename T, int HALVES> __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_constant__ TreeParams p) {
     extern __shared__ __align__(16) float smem[];
     grid_dependency_wait();
     grid_dependency_launch();
@@ -59,7 +60,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) tree_simt_kern
     const int D = p.head_dim, D4 = (D + 3) / 4 * 4, stride = D4 + 4;
     float *q_s = smem, *k_s = q_s + kRows * stride, *v_s = k_s + kTokens * stride, *p_s = v_s + kTokens * stride;
     float *m_s = p_s + kRows * (kTokens + 1), *l_s = m_s + kRows, *a_s = l_s + kRows;
-    __shared__ int64_t row_s[kTokens];
+    __shared__ int on_s[kTokens];  // whether the token is there
     const int tiles = (p.max_nodes * p.group + kRows - 1) / kRows;
     const int seq = blockIdx.z, kv_head = blockIdx.y / tiles, row0 = blockIdx.y % tiles * kRows, split = blockIdx.x;
     const TreeSequence s = span_of(p, seq);
@@ -68,13 +69,48 @@ template <typename T> __global__ void __launch_bounds__(kThreads) tree_simt_kern
     const int begin = (int)min((int64_t)split * p.chunk, (int64_t)s.tokens), end = (int)min((int64_t)begin + p.chunk, (int64_t)s.tokens);
     if (begin >= end && split > 0) return;  // the merge leaves it out
 
+    // K and V of a tile on their way: tokens rg + 8 i, dims cg * 4 (+ 64).  Asked for while the tile before is worked on, the first one
+    // while the queries are turned.
+    float4 k_next[HALVES][kTokens / 8], v_next[HALVES][kTokens / 8];
+    bool there[kTokens / 8];
+    auto request = [&](int t0) {
+        int64_t at[kTokens / 8];
+#pragma unroll
+        for (int i = 0; i < kTokens / 8; ++i) {
+            const int t = t0 + (tid >> 4) + 8 * i, logical = t / p.page_size;
+            at[i] = -1;
+            if (t < end) {
+                const int page = p.page_tables[(int64_t)seq * p.max_pages + logical];
+                if ((unsigned)page < (unsigned)p.physical_pages) {
+                    at[i] = (((int64_t)page * p.page_size + t - logical * p.page_size) * p.kv_heads + kv_head) * D;
+                } else if ((tid & 15) == 0) {  // never read: its tokens are left out and the call is flagged
+                    p.status->code = FLAT_ERR_PAGE_OUT_OF_RANGE;
+                    p.status->where = seq;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kTokens / 8; ++i) {
+            there[i] = at[i] >= 0;
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) {
+                const int e = (tid & 15) * 4 + h * 64;
+                k_next[h][i] = v_next[h][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (at[i] < 0 || e >= D) continue;
+                k_next[h][i] = load4<T>(static_cast<const T *>(p.k) + at[i] + e, p.vectors, D - e);
+                v_next[h][i] = load4<T>(static_cast<const T *>(p.v) + at[i] + e, p.vectors, D - e);
+            }
+        }
+    };
+    request(begin);
+
     // the rows' queries, turned, with the softmax scale and log2(e): scores come out in the exp2 domain
     const int rg = tid >> 4, cg = tid & 15;  // rows rg * 4 .. + 3; tokens cg, cg + 16; dims cg * 4 and cg * 4 + 64
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < HALVES; ++h) {
         const int e = cg * 4 + h * 64;
         if (e >= D4) break;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < kRows / 8; ++i) {
             const int r = rg + 8 * i;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -94,49 +130,26 @@ template <typename T> __global__ void __launch_bounds__(kThreads) tree_simt_kern
         m_s[tid] = -INFINITY;
         l_s[tid] = 0.f;
     }
-    float acc[4][8];
+    float acc[4][4 * HALVES];
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[r][e] = 0.f;
+        for (int e = 0; e < 4 * HALVES; ++e) acc[r][e] = 0.f;
 
     for (int t0 = begin; t0 < end; t0 += kTokens) {
         __syncthreads();
-        if (tid < kTokens) {
-            const int t = t0 + tid;
-            int64_t row = -1;
-            if (t < end) {
-                const int page = p.page_tables[(int64_t)seq * p.max_pages + t / p.page_size];
-                if ((unsigned)page < (unsigned)p.physical_pages) {
-                    row = (int64_t)page * p.page_size + t % p.page_size;
-                } else {  // never read: its tokens are left out and the call is flagged
-                    p.status->code = FLAT_ERR_PAGE_OUT_OF_RANGE;
-                    p.status->where = seq;
-                }
-            }
-            row_s[tid] = row;
-        }
-        __syncthreads();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int e = cg * 4 + h * 64;
-            if (e >= D4) break;
-            float4 k[kTokens / 8], v[kTokens / 8];
+        for (int i = 0; i < kTokens / 8; ++i) {
+            if (cg == 0) on_s[rg + 8 * i] = there[i];
 #pragma unroll
-            for (int i = 0; i < kTokens / 8; ++i) {
-                const int64_t row = row_s[rg + 8 * i];
-                k[i] = v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (row < 0) continue;
-                const int64_t at = (row * p.kv_heads + kv_head) * D + e;
-                k[i] = load4<T>(static_cast<const T *>(p.k) + at, p.vectors, D - e);
-                v[i] = load4<T>(static_cast<const T *>(p.v) + at, p.vectors, D - e);
-            }
-#pragma unroll
-            for (int i = 0; i < kTokens / 8; ++i) {
-                *reinterpret_cast<float4 *>(k_s + (rg + 8 * i) * stride + e) = k[i];
-                *reinterpret_cast<float4 *>(v_s + (rg + 8 * i) * stride + e) = v[i];
+            for (int h = 0; h < HALVES; ++h) {
+                const int e = cg * 4 + h * 64;
+                if (e >= D4) break;
+                *reinterpret_cast<float4 *>(k_s + (rg + 8 * i) * stride + e) = k_next[h][i];
+                *reinterpret_cast<float4 *>(v_s + (rg + 8 * i) * stride + e) = v_next[h][i];
             }
         }
+        if (t0 + kTokens < end) request(t0 + kTokens);
         __syncthreads();
         float x[4][2];
 #pragma unroll
@@ -158,7 +171,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) tree_simt_kern
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int t = cg + 16 * c;
-                on[c] = row < rows && row_s[t] >= 0 && sees(p, s, node, t0 + t);
+                on[c] = row < rows && on_s[t] && sees(p, s, node, t0 + t);
                 if (!on[c]) x[r][c] = -INFINITY;
             }
             float top = fmaxf(x[r][0], x[r][1]);
@@ -187,24 +200,24 @@ template <typename T> __global__ void __launch_bounds__(kThreads) tree_simt_kern
         for (int r = 0; r < 4; ++r) {
             const float a = a_s[rg * 4 + r];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[r][e] *= a;
+            for (int e = 0; e < 4 * HALVES; ++e) acc[r][e] *= a;
         }
         for (int t = 0; t < kTokens; ++t) {
-            float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
-            if (cg * 4 < D4) v0 = *reinterpret_cast<const float4 *>(v_s + t * stride + cg * 4);
-            if (cg * 4 + 64 < D4) v1 = *reinterpret_cast<const float4 *>(v_s + t * stride + cg * 4 + 64);
+            float4 v[HALVES];
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+                v[h] = cg * 4 + h * 64 < D4 ? *reinterpret_cast<const float4 *>(v_s + t * stride + cg * 4 + h * 64) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float w = p_s[(rg * 4 + r) * (kTokens + 1) + t];
                 if (w < 0.f) continue;
-                acc[r][0] = fmaf(w, v0.x, acc[r][0]);
-                acc[r][1] = fmaf(w, v0.y, acc[r][1]);
-                acc[r][2] = fmaf(w, v0.z, acc[r][2]);
-                acc[r][3] = fmaf(w, v0.w, acc[r][3]);
-                acc[r][4] = fmaf(w, v1.x, acc[r][4]);
-                acc[r][5] = fmaf(w, v1.y, acc[r][5]);
-                acc[r][6] = fmaf(w, v1.z, acc[r][6]);
-                acc[r][7] = fmaf(w, v1.w, acc[r][7]);
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h) {
+                    acc[r][4 * h] = fmaf(w, v[h].x, acc[r][4 * h]);
+                    acc[r][4 * h + 1] = fmaf(w, v[h].y, acc[r][4 * h + 1]);
+                    acc[r][4 * h + 2] = fmaf(w, v[h].z, acc[r][4 * h + 2]);
+                    acc[r][4 * h + 3] = fmaf(w, v[h].w, acc[r][4 * h + 3]);
+                }
             }
         }
     }
@@ -219,7 +232,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) tree_simt_kern
         const int64_t out = (int64_t)(s.first + (row0 + row) / p.group) * p.q_heads + kv_head * p.group + (row0 + row) % p.group;
         const int64_t part = (int64_t)split * p.max_q * p.q_heads + out;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 4 * HALVES; ++e) {
             const int d = cg * 4 + (e & 3) + (e >> 2) * 64;
             if (d >= D) continue;
             const float o = empty ? 0.f : acc[r][e] * inv;
@@ -263,15 +276,30 @@ template <typename T> __global__ void __launch_bounds__(128) tree_merge_kernel(c
     __syncwarp();
     const bool empty = sum == 0.f;
     const float inv = empty ? 0.f : 1.0f / sum;
-    for (int d = lane; d < D; d += 32) {
-        float o = 0.f;
+    // four dims a lane; lanes that are left take every second (fourth, ..) chunk
+    int width = 1;
+    while (width * 4 < D) width *= 2;
+    const int groups = 32 / width, d = lane % width * 4;
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    if (d < D) {
+        const bool vec = D % 4 == 0;  // the partial results' rows then are whole groups of four
 #pragma unroll 8
-        for (int i = 0; i < parts; ++i) {
-            const float x = p.partial_o[(i * rows + row) * D + d];
-            o = fmaf(w[i], x, o);  // a chunk in which the row sees nothing holds zeros
+        for (int i = lane / width; i < parts; i += groups) {
+            const float4 x = load4<float>(p.partial_o + (i * rows + row) * D + d, vec, D - d);
+            const float f = w[i];
+            o[0] = fmaf(f, x.x, o[0]);  // a chunk in which the row sees nothing holds zeros
+            o[1] = fmaf(f, x.y, o[1]);
+            o[2] = fmaf(f, x.z, o[2]);
+            o[3] = fmaf(f, x.w, o[3]);
         }
-        static_cast<T *>(p.o)[row * D + d] = from_float<T>(o * inv);
     }
+    for (int g = 16; g >= width; g /= 2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor_sync(0xffffffffu, o[e], g);
+    if (lane < width)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < D) static_cast<T *>(p.o)[row * D + d + e] = from_float<T>(o[e] * inv);
     if (lane == 0) p.lse[row] = empty ? -INFINITY : base + logf(sum);
 }
 
@@ -292,10 +320,11 @@ template <typename T> int launch(flat_ctx *ctx, TreeParams &p) {
     const int stride = (p.head_dim + 3) / 4 * 4 + 4;
     const size_t smem = ((kRows + 2 * kTokens) * stride + kRows * (kTokens + 1) + 3 * kRows) * sizeof(float);
     static_assert((32 + 64) * (kMaxHeadDim + 4) * 4 + 32 * 33 * 4 + 96 * 4 < 64 << 10, "shared memory of the largest head_dim");
-    FLAT_CUDA_OK(ctx, cudaFuncSetAttribute(tree_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 << 10));
+    auto *kernel = p.head_dim <= 64 ? tree_simt_kernel<T, 1> : tree_simt_kernel<T, 2>;
+    if (smem > 40 << 10) FLAT_CUDA_OK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 << 10));
     {
         KernelTimer timer(ctx);
-        FLAT_CUDA_OK(ctx, launch_dependent(may_overlap_previous(ctx), tree_simt_kernel<T>, dim3((unsigned)p.splits, (unsigned)(tiles * p.kv_heads), (unsigned)p.num_seqs),
+        FLAT_CUDA_OK(ctx, launch_dependent(may_overlap_previous(ctx), kernel, dim3((unsigned)p.splits, (unsigned)(tiles * p.kv_heads), (unsigned)p.num_seqs),
                                            kThreads, smem, ctx->stream, p));
     }
     ctx->launches += 1;

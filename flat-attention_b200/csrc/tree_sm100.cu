@@ -48,7 +48,7 @@ constexpr int kPoisonRing = 16;  // segments between the fixing warp and the slo
 template <int D, int ROWS> struct Cfg {
     static constexpr int kSoftmaxWarps = ROWS / 32, kQWarp = kSoftmaxWarps, kKWarp = kQWarp + kQWarps, kVWarp = kKWarp + 1, kMmaWarp = kVWarp + 1;
     static constexpr int kThreads = (kMmaWarp + 2) * 32;  // the last warp goes over V tiles
-    static constexpr int kQSteps = ROWS == 64 ? 4 : 2;    // tokens of a thread of the query warps in flight
+    static constexpr int kQSteps = ROWS == 64 ? 4 : 3;    // tokens of a thread of the query warps in flight, as many as the registers hold
     static constexpr int kBoxes = D / 64;
     static constexpr int kQBox = ROWS * 128, kQTile = kQBox * kBoxes;  // one of the two summands of the queries
     static constexpr int kGroup = 1024 * kBoxes;                        // 8 tokens
@@ -534,22 +534,19 @@ __global__ void __launch_bounds__((ROWS / 32 + 6) * 32, kCtasPerSm) tree_sm100_k
             // loads of 64 rows (of groups of four) are in flight while the last scores of the segment before are formed.
             uint4 raw[kQSteps][4];
             int position[kQSteps];
-            auto request = [&](int base) {
+            auto request = [&](int i, uint4 (&x)[4], int &at) {
+                if (i >= tasks) return;
+                const int nq = i / (D / 8), node = quads == 1 ? nq : nq / quads, h = (nq - node * quads) * 4;
+                at = p.t.positions[first + node];
+                const char *from = static_cast<const char *>(p.t.q) + (((int64_t)(first + node) * p.t.q_heads + head0 + h) * D + c * 8) * 2;
 #pragma unroll
-                for (int u = 0; u < kQSteps; ++u) {
-                    const int i = base + u * kQWarps * 32;
-                    if (i >= tasks) break;
-                    const int nq = i / (D / 8), node = quads == 1 ? nq : nq / quads, h = (nq - node * quads) * 4;
-                    position[u] = p.t.positions[first + node];
-                    const char *from = static_cast<const char *>(p.t.q) + (((int64_t)(first + node) * p.t.q_heads + head0 + h) * D + c * 8) * 2;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (h + e < p.t.group && (unsigned)(node * p.t.group + h + e - row0) < (unsigned)rows) raw[u][e] = *reinterpret_cast<const uint4 *>(from + e * D * 2);
-                }
+                for (int e = 0; e < 4; ++e)
+                    if (h + e < p.t.group && (unsigned)(node * p.t.group + h + e - row0) < (unsigned)rows) x[e] = *reinterpret_cast<const uint4 *>(from + e * D * 2);
             };
             const bool planning = k > 0 && more;
             if (planning) plan();
-            request(tid);
+#pragma unroll
+            for (int u = 0; u < kQSteps; ++u) request(tid + u * kQWarps * 32, raw[u], position[u]);
             if (k > 0) {
                 if (!mbar_wait_warp(q_empty, (k - 1) & 1, abort_flag)) {
                     if (lane == 0) record_timeout(p, 330);
@@ -565,7 +562,7 @@ __global__ void __launch_bounds__((ROWS / 32 + 6) * 32, kCtasPerSm) tree_sm100_k
                 if (lane == 0) mbar_arrive(go);
             }
 #pragma unroll 1
-            for (int i = tid, step = 0; i < tasks; i += kQWarps * 32) {
+            for (int i = tid; i < tasks; i += kQWarps * 32) {
                 const int nq = i / (D / 8), node = quads == 1 ? nq : nq / quads, h = (nq - node * quads) * 4;
                 float2 cs[4];
 #pragma unroll
@@ -579,17 +576,13 @@ __global__ void __launch_bounds__((ROWS / 32 + 6) * 32, kCtasPerSm) tree_sm100_k
                     if ((unsigned)r < (unsigned)rows) write_query<C::kQTile>(raw[0][0], cs, q_s + (c >> 3) * C::kQBox + r * 128 + (((c & 7) ^ (r & 7)) << 4));
                     raw[0][0] = raw[0][1], raw[0][1] = raw[0][2], raw[0][2] = raw[0][3];  // registers move so that the loops stay loops
                 }
-                if (++step == kQSteps) {
-                    step = 0;
-                    request(i + kQWarps * 32);
-                } else {
 #pragma unroll
-                    for (int u = 0; u + 1 < kQSteps; ++u) {
-                        position[u] = position[u + 1];
+                for (int u = 0; u + 1 < kQSteps; ++u) {
+                    position[u] = position[u + 1];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) raw[u][e] = raw[u + 1][e];
-                    }
+                    for (int e = 0; e < 4; ++e) raw[u][e] = raw[u + 1][e];
                 }
+                request(i + kQSteps * kQWarps * 32, raw[kQSteps - 1], position[kQSteps - 1]);
             }
             fence_proxy_async();
             __syncwarp();
