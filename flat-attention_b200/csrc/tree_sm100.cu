@@ -1,7 +1,7 @@
 // Attention of drafted tokens over a paged cache on the tensor cores: bf16, head_dim 64 or 128, pages of a multiple of 16 tokens.
 //
 //   rows of one (sequence, KV head): (drafted token, head of the group), n * G of them, all against the same keys and values
-//   S = Q K^T (SS MMA, 128 rows x 64 tokens)  ->  P = exp2(S - m)  ->  O += P V (A operand from TMEM)
+//   S = Q K^T (SS MMA, 64 or 128 rows x 64 tokens)  ->  P = exp2(S - m)  ->  O += P V (A operand from TMEM)
 //
 // Bound by the bytes of K and V, read once, and with hundreds of rows by the products; either way what counts is that nothing stands between
 // two tiles.  The beginning and the end of an item (queries read, turned and written; the first scores; the last weights; results) are
@@ -10,15 +10,16 @@
 //   K and V tiles of 64 tokens come by TMA, a box per page or tile, through a ring that runs on whatever item is at hand;
 //   one warp plans: it walks the span two items ahead of the products and puts what the other warps have to know in shared memory;
 //   two warps make the next item's queries as soon as the last scores of the item before are formed;
-//   ROWS / 32 warps work a softmax row per thread, without shuffles, and write results, while the next item's first scores are formed;
+//   four warps work a softmax row per thread, without shuffles, and write results, while the next item's first scores are formed;
 //   one thread issues all products.  Two score tiles alternate; P lies over the scores it comes from, and the products of one
 //   thread execute in order, so the scores after next cannot overtake the product that reads that P.
-// ROWS is 64 where no sequence has more (the ring takes the queries' place; half the rows of a product are whatever lies behind the
-// queries in shared memory: a product of 64 rows takes as long), otherwise 128.  Of more than 128 rows, two blocks of 128 go to two CTAs
-// that walk the same span, so that the second one finds K and V in the L2.
+// ROWS is 64 where no sequence has more, otherwise 128.  A product of 64 rows takes as long as one of 128, but half the power, and the
+// power limit is what a long run meets: one drafted token against 32 x 4000 takes 94 us a call in a run of seconds, with products
+// of 128 rows 119 (alone 91 and 98).  For the same reason rows that are not there are zeros.  Of more than 128 rows, two blocks of 128
+// go to two CTAs that walk the same span, so that the second one finds K and V in the L2.
 //
-// Work: the tiles of all items, a block of ROWS rows of a (sequence, KV head) each, stand in one line, which is cut into equal spans, one per CTA, whatever
-// the lengths are.  Every CTA adds the lengths up itself, so nothing is planned on the host.  An item that a span's end cuts is
+// Work: the tiles of all items, a block of ROWS rows of a (sequence, KV head) each, stand in one line, which is cut into equal spans,
+// one per CTA, whatever the lengths are.  Every CTA adds the lengths up itself, so nothing is planned on the host.  An item that a span's end cuts is
 // joined, from the parts in order, by the CTA that finds that they are all there; everything else is written directly.
 //
 // Roundings: q enters as the sum of two bf16 numbers (the tensor core takes one type, and K is bf16; q alone would cost 2^-9 of the
@@ -39,6 +40,7 @@ using namespace tree_tc;
 
 constexpr int kTok = 64, kAhead = 2;  // kAhead: score tiles
 constexpr int kQWarps = 2, kCtasPerSm = 2;
+constexpr int kThreads = 320;  // warps: softmax 4, queries 2, K, V, products, and one that goes over V tiles
 constexpr int kSegRing = 4;      // see below, planning
 constexpr int kValidRing = 16;   // tiles between the producer and the slowest softmax warp: the ring's and four more
 constexpr int kPoisonRing = 16;  // segments between the fixing warp and the slowest softmax warp
@@ -46,16 +48,15 @@ constexpr int kPoisonRing = 16;  // segments between the fixing warp and the slo
 // A K or V tile lies in shared memory as [8 tokens][64 dims of D][token of the 8][64 dims]: one TMA box of any number of tokens
 // then writes all D dims.  Queries: [summand][64 dims of D][row][64 dims].
 template <int D, int ROWS> struct Cfg {
-    static constexpr int kSoftmaxWarps = ROWS / 32, kQWarp = kSoftmaxWarps, kKWarp = kQWarp + kQWarps, kVWarp = kKWarp + 1, kMmaWarp = kVWarp + 1;
-    static constexpr int kThreads = (kMmaWarp + 2) * 32;  // the last warp goes over V tiles
-    static constexpr int kQSteps = ROWS == 64 ? 4 : 3;    // tokens of a thread of the query warps in flight, as many as the registers hold
+    static constexpr int kSoftmaxWarps = 4, kWarpRows = ROWS / 4, kQWarp = kSoftmaxWarps, kKWarp = kQWarp + kQWarps, kVWarp = kKWarp + 1, kMmaWarp = kVWarp + 1;
+    static constexpr int kQSteps = 3;                     // tokens of a thread of the query warps in flight, as many as the registers hold
     static constexpr int kBoxes = D / 64;
     static constexpr int kQBox = ROWS * 128, kQTile = kQBox * kBoxes;  // one of the two summands of the queries
     static constexpr int kGroup = 1024 * kBoxes;                        // 8 tokens
     static constexpr int kKvTile = kTok / 8 * kGroup;
     static constexpr int kControl = 1024, kSmem = (228 / kCtasPerSm - 1) * 1024;  // of an SM's 228 KB, 1 KB a CTA is the system's
     static constexpr int kStages = (kSmem - kControl - 2 * kQTile) / kKvTile;     // D = 128: 5 and 3, D = 64: 12 and 10
-    static_assert(2 * kQTile - kQBox + kMmaRows * 128 <= 2 * kQTile + kStages * kKvTile, "what a product reads behind the queries");
+    static_assert(kStages >= 3 && 4 * kStages + 9 + kSegRing <= 64, "ring");
 };
 
 struct KernelParams {
@@ -211,12 +212,12 @@ template <int D, int ROWS> __device__ __forceinline__ void join_parts(const Kern
 }
 
 template <int D, int ROWS>
-__global__ void __launch_bounds__((ROWS / 32 + 6) * 32, kCtasPerSm) tree_sm100_kernel(const __grid_constant__ KernelParams p) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const __grid_constant__ KernelParams p) {
     using C = Cfg<D, ROWS>;
     using Ctl = Control<ROWS, C::kStages>;
     constexpr int kSoftmaxWarps = C::kSoftmaxWarps, kQWarp = C::kQWarp, kKWarp = C::kKWarp, kVWarp = C::kVWarp, kMmaWarp = C::kMmaWarp;
-    constexpr int kThreads = C::kThreads, kQSteps = C::kQSteps;
-    static_assert(kThreads == (ROWS / 32 + 6) * 32, "launch bounds");
+    constexpr int kQSteps = C::kQSteps;
+    static_assert(kThreads == (kMmaWarp + 2) * 32, "warps");
     extern __shared__ __align__(1024) uint8_t smem[];
     Ctl &ctl = *reinterpret_cast<Ctl *>(smem);
     static_assert(sizeof(Ctl) <= C::kControl, "control block");
@@ -265,6 +266,9 @@ __global__ void __launch_bounds__((ROWS / 32 + 6) * 32, kCtasPerSm) tree_sm100_k
         tmem_alloc(smem_u32(&ctl.tmem), 512 / kCtasPerSm);
         tmem_relinquish();
     }
+    // rows that are not there are zeros, see above
+    for (int i = threadIdx.x; i < 2 * C::kQTile / 16; i += kThreads) reinterpret_cast<uint4 *>(q_s)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async();
     grid_dependency_wait();
     grid_dependency_launch();
 
@@ -338,13 +342,14 @@ __global__ void __launch_bounds__((ROWS / 32 + 6) * 32, kCtasPerSm) tree_sm100_k
     } else if (warp < kSoftmaxWarps) {
         // ================= softmax and results =================
         const uint32_t lanes = (uint32_t)warp << 21;  // this warp's quarter of the TMEM lanes
-        const int row = threadIdx.x;
+        // The accumulator's rows lie in lanes 0 .. 31 of each quarter of the TMEM lanes, of 64 rows in lanes 0 .. 15.
+        const int row = lane < C::kWarpRows ? warp * C::kWarpRows + lane : ROWS;
         int count = 0;  // tiles so far
         for (int k = 0;; ++k) {
             const Segment &g = segment(k);
             if (!ok || g.n == 0) break;
             const int rows = g.rows, n = g.n, j0 = g.j0, len = g.s.len;
-            const bool live = row < rows, warp_live = warp * 32 < rows;
+            const bool live = row < rows, warp_live = warp * C::kWarpRows < rows;
             const int node = live ? (g.row0 + row) / p.t.group : 0;
             uint32_t own0 = 0, own1 = 0;  // first mask bits
             if (p.t.mask && live) {
@@ -411,6 +416,9 @@ __global__ void __launch_bounds__((ROWS / 32 + 6) * 32, kCtasPerSm) tree_sm100_k
                         }
                     }
                     const float base = m == -INFINITY ? 0.f : m;
+                    if (!live)  // P = 0
+#pragma unroll
+                        for (int e = 0; e < kTok; ++e) x[e] = 0xff800000u;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -760,8 +768,8 @@ template <int D, int ROWS> int launch(flat_ctx *ctx, const TreeParams &t) {
     const uint64_t rows = (uint64_t)t.physical_pages * t.page_size;
     if (int st = make_pool_map(ctx, &p.map_k, t.k, D, rows, t.kv_heads, p.box_rows)) return st;
     if (int st = make_pool_map(ctx, &p.map_v, t.v, D, rows, t.kv_heads, p.box_rows)) return st;
-    p.idesc_qk = make_idesc(kFmtBF16, kFmtBF16, 0, 0, kMmaRows, kTok);
-    p.idesc_pv = make_idesc(kFmtBF16, kFmtBF16, 0, 1, kMmaRows, D);
+    p.idesc_qk = make_idesc(kFmtBF16, kFmtBF16, 0, 0, ROWS, kTok);
+    p.idesc_pv = make_idesc(kFmtBF16, kFmtBF16, 0, 1, ROWS, D);
     const int grid = ctx->sm_count * kCtasPerSm;
     static_assert(kCtasPerSm == 2, "the grid has to be even");
     char *at = static_cast<char *>(ctx->paged_scratch) + kPagedPlanBytes;
@@ -775,7 +783,7 @@ template <int D, int ROWS> int launch(flat_ctx *ctx, const TreeParams &t) {
     FLAT_CUDA_OK(ctx, cudaFuncSetAttribute(tree_sm100_kernel<D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     {
         KernelTimer timer(ctx);
-        FLAT_CUDA_OK(ctx, launch_dependent(may_overlap_previous(ctx), tree_sm100_kernel<D, ROWS>, dim3((unsigned)grid), C::kThreads, C::kSmem, ctx->stream, p));
+        FLAT_CUDA_OK(ctx, launch_dependent(may_overlap_previous(ctx), tree_sm100_kernel<D, ROWS>, dim3((unsigned)grid), kThreads, C::kSmem, ctx->stream, p));
     }
     ctx->launches += 1;
     return FLAT_OK;
