@@ -620,9 +620,10 @@ int32_t flat_splitkv_merge(flat_ctx *ctx, int32_t dtype, uint64_t parts, uint64_
  * captured in a CUDA graph and replayed; the host gives upper bounds.  All of them enqueue on the context's stream.
  * Their scratch (48 MiB) is allocated by the first of them that is made on a context and never moves: make one call
  * before a stream capture.  It is used in stream order, so graphs captured on one context must not run at the same
- * time; two contexts have nothing in common.  What the host cannot see is checked on the device: a sequence whose
- * entries make no sense is left out (as each call says) and flat_ctx_device_status reports it.  No counterpart in the
- * reference, whose paged caches hold one sequence and whose page table is host data (src/paged_kv.rs:75-188). */
+ * time; two contexts have nothing in common.  A page belongs to one sequence: release puts it on the stack whoever else
+ * names it.  What the host cannot see is checked on the device: a sequence whose entries make no sense is left out (as
+ * each call says) and flat_ctx_device_status reports it.  No counterpart in the reference, whose paged caches hold one
+ * sequence and whose page table is host data (src/paged_kv.rs:75-188). */
 typedef struct flat_paged_batch {
     uint64_t num_seqs;          /* at most 65535 */
     uint64_t page_size;         /* tokens of a page */
@@ -645,7 +646,7 @@ typedef struct flat_paged_batch {
  * last token, get slot -1 and position 0.  page_counts_out [num_seqs], free_count_out [1] (null: in place) receive the
  * counts afterwards, context_lens_out (null: not written; may be context_lens) context_lens + new_lens of served sequences.
  * Device status: CAPACITY_EXCEEDED (a sequence was refused for want of pages), INVALID_CACHE_LENGTH (negative lengths, more
- * live tokens than its pages hold, more than max_pages_per_seq pages or more than max_new_tokens tokens),
+ * live tokens than its pages hold, more than max_pages_per_seq pages, 2^31 - 1 or max_new_tokens tokens),
  * PAGE_OUT_OF_RANGE (an entry outside the pool; its tokens get slot -1), CAPACITY_OVERFLOW (free_count outside the pool). */
 int32_t flat_paged_batch_reserve(flat_ctx *ctx, const flat_paged_batch *batch, const int32_t *new_lens_dev,
                                  const int32_t *depths_dev, uint64_t max_new_tokens, int32_t *page_counts_out,
@@ -680,6 +681,7 @@ int32_t flat_paged_kv_write(flat_ctx *ctx, int32_t dtype, uint64_t tokens, uint6
  * [O(max_q_tokens*q_heads*head_dim) | LSE(max_q_tokens*q_heads)] (flat_decode_layout_for with batch = max_q_tokens); rows behind
  * q_offsets[num_seqs] are left as they are.  A token that sees nothing gets O = 0, LSE = -inf.  K and V of tokens that a row does not
  * see have no influence on it, NaN and infinities among them.  Results are bitwise repeatable for the same lengths and bounds.
+ * max_nodes * q_heads / kv_heads is at most 2^24.
  * Device status: LENGTH_MISMATCH (offsets that fall or leave Q, more than max_nodes drafted tokens, a negative length: the
  * sequence's rows are not written), PAGE_OUT_OF_RANGE (tokens without a page of the pool, or behind max_context: left out). */
 int32_t flat_decode_paged_tree(flat_ctx *ctx, int32_t dtype, const flat_paged_batch *batch, uint64_t q_heads,
