@@ -503,10 +503,12 @@ class Context:
         k_source / v_source [tokens, kv_heads*head_dim], k / v [pool_rows, kv_heads*head_dim]."""
         tokens = slot_map.numel()
         _ints(tokens, slot_map=slot_map, positions=positions)
-        dtype, pool = _same_type(k_source, v_source, k, v), _whole(k)
-        pool_rows = pool.bytes // (kv_heads * head_dim * k_source.element_size()) if kv_heads * head_dim else 0
-        self.check(lib().flat_paged_kv_write(self.h, dtype, tokens, kv_heads, head_dim, pool_rows, _p(slot_map), _p(positions),
-                                             theta, _whole(k_source), _whole(v_source), pool, _whole(v)))
+        dtype, buffers = _buffers(k_source, v_source, k, v)
+        if dtype is None:
+            raise FlatAttentionError(26, "one of the tensors has to tell the type")
+        row = kv_heads * head_dim * (4 if dtype == F32 else 2)
+        pool_rows = buffers[2].bytes // row if row else 0
+        self.check(lib().flat_paged_kv_write(self.h, dtype, tokens, kv_heads, head_dim, pool_rows, _p(slot_map), _p(positions), theta, *buffers))
 
     def decode_paged_tree(self, batch: "PagedBatch", q_heads: int, kv_heads: int, head_dim: int, max_nodes: int, max_context: int, q_offsets,
                           q_positions, tree_mask, cfg, theta: float, q, k, v, out):
@@ -522,9 +524,10 @@ class Context:
                 raise FlatAttentionError(7, f"tree_mask has shape {tuple(tree_mask.shape)}, expected [{tokens}, words]")
             words = tree_mask.shape[1]
             _ints(tokens * words, tree_mask=tree_mask)
-        self.check(lib().flat_decode_paged_tree(self.h, _same_type(q, k, v), batch.ref, q_heads, kv_heads, head_dim, tokens, max_nodes, max_context,
-                                                _p(q_offsets), _p(q_positions), _p(tree_mask), words, C.byref(cfg), theta, _whole(q), _whole(k),
-                                                _whole(v), _whole(out)))
+        dtype, buffers = _buffers(q, k, v)
+        self.check(lib().flat_decode_paged_tree(self.h, batch.dtype if dtype is None else dtype, batch.ref, q_heads, kv_heads, head_dim, tokens, max_nodes,
+                                                max_context, _p(q_offsets), _p(q_positions), _p(tree_mask), words, C.byref(cfg), theta, *buffers,
+                                                _whole(out)))
 
     def paged_kv_accept(self, batch: "PagedBatch", kv_heads: int, head_dim: int, accept_nodes, accept_lens, context_lens_out, k, v):
         """Moves the rows of each sequence's accepted path (accept_nodes [num_seqs, max_accept], the first accept_lens[s] of a row) behind
@@ -533,9 +536,9 @@ class Context:
             raise FlatAttentionError(7, f"accept_nodes has shape {tuple(accept_nodes.shape)}, expected [{batch.num_seqs}, max_accept]")
         _ints(accept_nodes.numel(), accept_nodes=accept_nodes)
         _ints(batch.num_seqs, accept_lens=accept_lens, context_lens_out=context_lens_out)
-        dtype = _same_type(k, v)
+        dtype, buffers = _buffers(k, v)
         self.check(lib().flat_paged_kv_accept(self.h, batch.dtype if dtype is None else dtype, batch.ref, kv_heads, head_dim,
-                                              accept_nodes.shape[1], _p(accept_nodes), _p(accept_lens), _p(context_lens_out), _whole(k), _whole(v)))
+                                              accept_nodes.shape[1], _p(accept_nodes), _p(accept_lens), _p(context_lens_out), *buffers))
 
     def chunked_prefill(self, dtype, shp, cfg, rot, query_chunk_size, q, k, v, out):
         self.check(lib().flat_chunked_prefill(self.h, C.c_int32(dtype), C.byref(shp), C.byref(cfg), C.byref(rot),
@@ -655,23 +658,24 @@ def _ints(elements: int, **tensors):
         raise FlatAttentionError(22, f"{name} has {t.numel()} elements, requires {elements}")
 
 
-def _same_type(*tensors):
-    """Tensors (flat_buffer views have no type) share one; returns its dtype code, None if all are views."""
-    first = None
-    for t in tensors:
-        if isinstance(t, Buffer):
-            continue
-        if first is None:
-            first = t.dtype
-            code = _dtype_of(t)
-        elif t.dtype is not first:
-            raise FlatAttentionError(26, "Q, K and V differ in type")
-    return None if first is None else code
+def _buffers(*tensors):
+    """(dtype code, flat_buffer of each): contiguous CUDA tensors of one type, or flat_buffer views, which have none (all views: None)."""
+    first, buffers = None, []
+    for x in tensors:
+        if type(x) is not Buffer:
+            dtype = x.dtype
+            if first is None:
+                first, code = dtype, _dtype_of(x)
+            elif dtype is not first:
+                raise FlatAttentionError(26, "Q, K and V differ in type")
+            x = _whole(x)
+        buffers.append(x)
+    return None if first is None else code, buffers
 
 
 def _whole(x) -> Buffer:
     """A contiguous CUDA tensor or a flat_buffer view."""
-    if isinstance(x, Buffer):
+    if type(x) is Buffer:
         return x
     if not x.is_cuda or not x.is_contiguous():
         raise FlatAttentionError(29, "tensors must be contiguous and on the device")
