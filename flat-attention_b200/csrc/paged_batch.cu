@@ -309,34 +309,16 @@ template <bool RELEASE> __global__ void __launch_bounds__(kScanThreads) paged_ba
         if ((threadIdx.x & 31) == 0 && given_out) atomicAdd(&taken_s, given_out);
         total = min(total, (int64_t)p.max_tokens);
     }
+    if (threadIdx.x == 0) starts_s[p.num_seqs] = (int)total;
+    __syncthreads();
+    // All reads of what may be written in place are done: the block's scan has used them.  The answer comes during the fill.
     if (threadIdx.x == 0) {
-        starts_s[p.num_seqs] = (int)total;
-        // all reads of what may be written in place are done: the block's scans have used them
         if (gridDim.x == 1) {
             last_s = 1;
         } else {
             __threadfence();
             last_s = atomicInc(p.plan_ticket, gridDim.x - 1) == gridDim.x - 1;
             __threadfence();
-        }
-    }
-    __syncthreads();
-    if (last_s) {
-#pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-            const int s = s0 + i;
-            if (i >= items || s >= p.num_seqs) break;
-            p.page_counts_out[s] = held[i];
-            if (!RELEASE) {
-                p.offsets[s] = starts_s[s];
-                if (p.context_lens_out) p.context_lens_out[s] = flags[i] == FLAT_OK ? L[i] + A[i] : L[i];
-            }
-            if (flags[i] != FLAT_OK) flag(p.status, flags[i], s);
-        }
-        if (threadIdx.x == 0) {
-            if (!RELEASE) p.offsets[p.num_seqs] = (int)total;
-            *p.free_count_out = RELEASE ? f + (int)total : f - taken_s;
-            if (f != given) flag(p.status, FLAT_ERR_CAPACITY_OVERFLOW, -1);
         }
     }
     // kItems tokens (pages) in a row for a thread: they mostly are the same sequence's, whose start is found once
@@ -382,6 +364,25 @@ template <bool RELEASE> __global__ void __launch_bounds__(kScanThreads) paged_ba
                     p.positions[i0 + u] = x[u].position;
                 }
             }
+        }
+    }
+    __syncthreads();
+    if (last_s) {
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const int s = s0 + i;
+            if (i >= items || s >= p.num_seqs) break;
+            p.page_counts_out[s] = held[i];
+            if (!RELEASE) {
+                p.offsets[s] = starts_s[s];
+                if (p.context_lens_out) p.context_lens_out[s] = flags[i] == FLAT_OK ? L[i] + A[i] : L[i];
+            }
+            if (flags[i] != FLAT_OK) flag(p.status, flags[i], s);
+        }
+        if (threadIdx.x == 0) {
+            if (!RELEASE) p.offsets[p.num_seqs] = (int)total;
+            *p.free_count_out = RELEASE ? f + (int)total : f - taken_s;
+            if (f != given) flag(p.status, FLAT_ERR_CAPACITY_OVERFLOW, -1);
         }
     }
 }

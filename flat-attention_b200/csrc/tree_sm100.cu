@@ -211,6 +211,11 @@ template <int D, int ROWS> __device__ __forceinline__ void join_parts(const Kern
     }
 }
 
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
 template <int D, int ROWS>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const __grid_constant__ KernelParams p) {
     using C = Cfg<D, ROWS>;
@@ -427,18 +432,32 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const 
                     if (!live)  // P = 0
 #pragma unroll
                         for (int e = 0; e < kTok; ++e) x[e] = 0xff800000u;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint64_t sum2 = 0, sum3 = 0;
+                    const uint64_t nbase = pack2(-base, -base);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
-                            const float pa = ex2(__uint_as_float(x[32 * h + e]) - base), pb = ex2(__uint_as_float(x[32 * h + e + 1]) - base);
-                            sum[(e >> 1) & 3] += pa + pb;
+                            float pa, pb;
+                            uint64_t t2, p2;
+                            asm("mov.b64 %0, {%1, %2};" : "=l"(t2) : "r"(x[32 * h + e]), "r"(x[32 * h + e + 1]));
+                            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(t2) : "l"(nbase));
+                            asm("mov.b64 {%0, %1}, %2;" : "=f"(pa), "=f"(pb) : "l"(t2));
+                            pa = ex2(pa);
+                            pb = ex2(pb);
+                            asm("mov.b64 %0, {%1, %2};" : "=l"(p2) : "f"(pa), "f"(pb));
+                            if (e & 2) asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum3) : "l"(p2));
+                            else asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum2) : "l"(p2));
                             x[32 * h + e / 2] = pack_bf16(pa, pb);
                         }
                         tmem_st16(tmem_base + lanes + col_s(b) + 16 * h, x + 32 * h);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    {
+                        float s0, s1, s2f, s3;
+                        asm("mov.b64 {%0, %1}, %2;" : "=f"(s0), "=f"(s1) : "l"(sum2));
+                        asm("mov.b64 {%0, %1}, %2;" : "=f"(s2f), "=f"(s3) : "l"(sum3));
+                        l += (s0 + s1) + (s2f + s3);
+                    }
                     tc_wait_st();
                     tc_fence_before();
                 }
