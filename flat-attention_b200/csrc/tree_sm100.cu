@@ -167,15 +167,16 @@ template <int D, int ROWS> __device__ __forceinline__ void join_parts(const Kern
     auto weight = [](float2 ml, float mx) { return ml.y == 0.f ? 0.f : ex2(ml.x - mx); };  // a part in which the row has seen nothing; a NaN counts
     float mx = -INFINITY, sum = 0.f;
 #pragma unroll 1
-    for (int base = 0; base < parts; base += 4) {
-        float2 ml[4];
+    for (int base = 0; base < parts; base += 8) {
+        float2 ml[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) ml[u] = base + u < parts ? __ldcg(&p.part_ml[part(base + u) * ROWS + r]) : make_float2(-INFINITY, 0.f);
+        for (int u = 0; u < 8; ++u) ml[u] = base + u < parts ? __ldcg(&p.part_ml[part(base + u) * ROWS + r]) : make_float2(-INFINITY, 0.f);
         const float before = mx;
-        mx = fmaxf(fmaxf(mx, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+#pragma unroll
+        for (int u = 0; u < 8; ++u) mx = fmaxf(mx, ml[u].x);
         sum *= before == -INFINITY ? 0.f : ex2(before - mx);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) sum = fmaf(weight(ml[u], mx), ml[u].y, sum);
+        for (int u = 0; u < 8; ++u) sum = fmaf(weight(ml[u], mx), ml[u].y, sum);
     }
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     const int row = item.row0 + r, node = row / p.t.group;
@@ -216,6 +217,7 @@ __device__ __forceinline__ uint64_t pack2(float a, float b) {
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
     return r;
 }
+
 template <int D, int ROWS>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const __grid_constant__ KernelParams p) {
     using C = Cfg<D, ROWS>;
