@@ -163,14 +163,14 @@ def lib() -> C.CDLL:
     return _lib
 
 
-_torch_module = None
+_torch_module = _int32 = None
 
 
 def _torch():
-    global _torch_module
+    global _torch_module, _int32
     if _torch_module is None:
         import torch
-        _torch_module = torch
+        _torch_module, _int32 = torch, torch.int32
     return _torch_module
 
 
@@ -485,30 +485,29 @@ class Context:
                             page_counts_out=None, free_count_out=None, context_lens_out=None):
         """Pages and slots for new_lens[s] tokens behind each sequence's live ones (flat_paged_batch_reserve); outputs None: in place,
         context_lens_out None: not written."""
-        _ints(batch.num_seqs, new_lens=new_lens, page_counts_out=page_counts_out, context_lens_out=context_lens_out)
-        _ints(max_new_tokens, slot_map=slot_map, positions=positions, depths=depths)
-        _ints(batch.num_seqs + 1, new_offsets=new_offsets)
-        _ints(1, free_count_out=free_count_out)
-        self.check(lib().flat_paged_batch_reserve(self.h, batch.ref, _p(new_lens), _p(depths), max_new_tokens, _p(page_counts_out),
-                                                  _p(free_count_out), _p(context_lens_out), _p(new_offsets), _p(slot_map), _p(positions)))
+        S, T = batch.num_seqs, max_new_tokens
+        self.check(lib().flat_paged_batch_reserve(
+            self.h, batch.ref, _ptr(new_lens, S, "new_lens"), _ptr(depths, T, "depths"), T, _ptr(page_counts_out, S, "page_counts_out"),
+            _ptr(free_count_out, 1, "free_count_out"), _ptr(context_lens_out, S, "context_lens_out"), _ptr(new_offsets, S + 1, "new_offsets"),
+            _ptr(slot_map, T, "slot_map"), _ptr(positions, T, "positions")))
 
     def paged_batch_release(self, batch: "PagedBatch", keep_lens, page_counts_out=None, free_count_out=None):
         """Gives back each sequence's pages behind its first keep_lens[s] tokens (flat_paged_batch_release)."""
-        _ints(batch.num_seqs, keep_lens=keep_lens, page_counts_out=page_counts_out)
-        _ints(1, free_count_out=free_count_out)
-        self.check(lib().flat_paged_batch_release(self.h, batch.ref, _p(keep_lens), _p(page_counts_out), _p(free_count_out)))
+        S = batch.num_seqs
+        self.check(lib().flat_paged_batch_release(self.h, batch.ref, _ptr(keep_lens, S, "keep_lens"), _ptr(page_counts_out, S, "page_counts_out"),
+                                                  _ptr(free_count_out, 1, "free_count_out")))
 
     def paged_kv_write(self, kv_heads: int, head_dim: int, slot_map, positions, theta: float, k_source, v_source, k, v):
         """New tokens' K (turned at `positions`; None: as it is) and V into the pool rows that slot_map names (flat_paged_kv_write).
         k_source / v_source [tokens, kv_heads*head_dim], k / v [pool_rows, kv_heads*head_dim]."""
         tokens = slot_map.numel()
-        _ints(tokens, slot_map=slot_map, positions=positions)
+        slots, at = _ptr(slot_map, tokens, "slot_map"), _ptr(positions, tokens, "positions")
         dtype, buffers = _buffers(k_source, v_source, k, v)
         if dtype is None:
             raise FlatAttentionError(26, "one of the tensors has to tell the type")
         row = kv_heads * head_dim * (4 if dtype == F32 else 2)
         pool_rows = buffers[2].bytes // row if row else 0
-        self.check(lib().flat_paged_kv_write(self.h, dtype, tokens, kv_heads, head_dim, pool_rows, _p(slot_map), _p(positions), theta, *buffers))
+        self.check(lib().flat_paged_kv_write(self.h, dtype, tokens, kv_heads, head_dim, pool_rows, slots, at, theta, *buffers))
 
     def decode_paged_tree(self, batch: "PagedBatch", q_heads: int, kv_heads: int, head_dim: int, max_nodes: int, max_context: int, q_offsets,
                           q_positions, tree_mask, cfg, theta: float, q, k, v, out):
@@ -516,17 +515,15 @@ class Context:
         them behind each sequence's live tokens (flat_decode_paged_tree).  tree_mask: int32 [tokens, words] of bits, or None.  `out`:
         create_decode_output_buffer(dtype, tokens, q_heads, head_dim)."""
         tokens = q_positions.numel()
-        _ints(batch.num_seqs + 1, q_offsets=q_offsets)
-        _ints(tokens, q_positions=q_positions)
+        offsets, at = _ptr(q_offsets, batch.num_seqs + 1, "q_offsets"), _ptr(q_positions, tokens, "q_positions")
         words = 0
         if tree_mask is not None:
             if tree_mask.dim() != 2 or tree_mask.shape[0] != tokens:
                 raise FlatAttentionError(7, f"tree_mask has shape {tuple(tree_mask.shape)}, expected [{tokens}, words]")
             words = tree_mask.shape[1]
-            _ints(tokens * words, tree_mask=tree_mask)
         dtype, buffers = _buffers(q, k, v)
         self.check(lib().flat_decode_paged_tree(self.h, batch.dtype if dtype is None else dtype, batch.ref, q_heads, kv_heads, head_dim, tokens, max_nodes,
-                                                max_context, _p(q_offsets), _p(q_positions), _p(tree_mask), words, C.byref(cfg), theta, *buffers,
+                                                max_context, offsets, at, _ptr(tree_mask, tokens * words, "tree_mask"), words, C.byref(cfg), theta, *buffers,
                                                 _whole(out)))
 
     def paged_kv_accept(self, batch: "PagedBatch", kv_heads: int, head_dim: int, accept_nodes, accept_lens, context_lens_out, k, v):
@@ -534,11 +531,11 @@ class Context:
         its live tokens and lengthens it (flat_paged_kv_accept); context_lens_out None: in place."""
         if accept_nodes.dim() != 2 or accept_nodes.shape[0] != batch.num_seqs:
             raise FlatAttentionError(7, f"accept_nodes has shape {tuple(accept_nodes.shape)}, expected [{batch.num_seqs}, max_accept]")
-        _ints(accept_nodes.numel(), accept_nodes=accept_nodes)
-        _ints(batch.num_seqs, accept_lens=accept_lens, context_lens_out=context_lens_out)
+        S = batch.num_seqs
+        nodes = _ptr(accept_nodes, 0, "accept_nodes")
         dtype, buffers = _buffers(k, v)
         self.check(lib().flat_paged_kv_accept(self.h, batch.dtype if dtype is None else dtype, batch.ref, kv_heads, head_dim,
-                                              accept_nodes.shape[1], _p(accept_nodes), _p(accept_lens), _p(context_lens_out), *buffers))
+                                              accept_nodes.shape[1], nodes, _ptr(accept_lens, S, "accept_lens"), _ptr(context_lens_out, S, "context_lens_out"), *buffers))
 
     def chunked_prefill(self, dtype, shp, cfg, rot, query_chunk_size, q, k, v, out):
         self.check(lib().flat_chunked_prefill(self.h, C.c_int32(dtype), C.byref(shp), C.byref(cfg), C.byref(rot),
@@ -641,8 +638,13 @@ def _b(x) -> Buffer:
     return x if isinstance(x, Buffer) else buf(x)
 
 
-def _p(t):
-    return None if t is None else t.data_ptr()
+def _ptr(t, elements: int, name: str):
+    """Address of a contiguous int32 CUDA tensor of at least `elements`; None stays None."""
+    if t is None:
+        return None
+    if t.dtype is not _int32 or not t.is_cuda or not t.is_contiguous() or t.numel() < elements:
+        _ints(elements, **{name: t})
+    return t.data_ptr()
 
 
 def _ints(elements: int, **tensors):
