@@ -231,6 +231,34 @@ def test_a_captured_call_follows_the_lengths_on_the_device():
         del g
 
 
+@pytest.mark.parametrize("dtype", [fa.BF16, fa.F32])
+def test_a_pool_of_more_than_2_to_the_31_elements(dtype):
+    """The same rows at the pool's beginning and behind its 2^31-th element (byte offsets behind 2^32): written, attended and moved alike."""
+    Hq, Hkv, D, page = 16, 8, 128, 16
+    td = fa.torch_dtype(dtype)
+    pool = (2 ** 31 // (Hkv * D) + 4096) // page
+    k, v = (torch.empty(pool * page, Hkv * D, dtype=td, device="cuda") for _ in range(2))
+    t = TreeCase(41, dtype, Hq, Hkv, D, page, [300, 45], [9, 20])
+    c = ctx()
+    results = []
+    for at in (0, pool - t.pool):
+        rows = slice(at * page, (at + t.pool) * page)
+        k[rows], v[rows] = t.k.to(td).cuda(), t.v.to(td).cuda()
+        b = fa.PagedBatch(2, page, pool, t.most, i32(np.where(t.table < 0, -1, t.table + at)), i32(t.held), i32(t.lens), i32(np.zeros(pool)), i32([0]))
+        slots = i32(np.concatenate([t.row(s, np.arange(a, a + n)) for s, (a, n) in enumerate(zip(t.lens, t.nodes))]) + at * page)
+        new = [torch.randn(t.T, Hkv * D, generator=torch.Generator().manual_seed(7)).to(td).cuda() for _ in range(2)]
+        c.paged_kv_write(Hkv, D, slots, i32(t.positions), THETA, new[0], new[1], k, v)
+        out = c.create_decode_output_buffer(dtype, t.rows, Hq, D)
+        out.fill_(0)
+        c.decode_paged_tree(b, Hq, Hkv, D, 20, 400, i32(t.offsets), i32(t.positions), None, fa.config(True), THETA, t.q.to(td).cuda(), k, v, out)
+        c.paged_kv_accept(b, Hkv, D, i32([[0, 2, 7], [5, 19, -1]]), i32([3, 2]), None, k, v)
+        clean(c)
+        results.append((out.cpu(), k[rows].cpu(), v[rows].cpu(), b.context_lens.cpu()))
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
+    assert not torch.equal(results[0][1], t.k.to(td)) and results[0][3].tolist() == [303, 47]
+
+
 def test_refusals_of_more_rows_than_a_launch_takes():
     b = fa.PagedBatch(1, 16, 4, 4)
     t = lambda n: torch.zeros(n, dtype=torch.bfloat16, device="cuda")  # noqa: E731
