@@ -65,6 +65,7 @@ struct KernelParams {
     uint32_t idesc_qk, idesc_pv;
     int box_rows;      // tokens of a TMA box: 16, 32 or 64, a divisor of the page size
     int share;         // CTAs of a span: 2 where two blocks of rows share K and V
+    int items;         // of the line, at most
     float4 *part_o;    // [2 per CTA][D / 4][ROWS], not normalised
     float2 *part_ml;   // [2 per CTA][ROWS] maximum (log2 domain) and sum
     unsigned *arrived; // [CTA]: warps that have written their part of the item that begins in this CTA and ends in a later one; 0 between calls
@@ -81,14 +82,16 @@ struct Segment {
 
 __device__ __forceinline__ int tiles_of(const TreeSequence &s) { return max(1, (s.tokens + kTok - 1) / kTok); }
 template <int ROWS> __device__ __forceinline__ int blocks_of(const TreeParams &p, const TreeSequence &s) { return (s.nodes * p.group + ROWS - 1) / ROWS; }
-// What a sequence takes of the line: the tiles of its items, or of its pairs of items where two CTAs walk a span.
-template <int ROWS> __device__ __forceinline__ int units_of(const KernelParams &p, const TreeSequence &s) {
-    return s.nodes == 0 ? 0 : (blocks_of<ROWS>(p.t, s) * p.t.kv_heads + p.share - 1) / p.share * tiles_of(s);
+// An item's place on the line, in tiles: whole multiples of `grain`.
+__device__ __forceinline__ int pitch_of(int tiles, int grain) { return (int)(((unsigned)tiles + (unsigned)grain - 1) / (unsigned)grain) * grain; }
+// What a sequence takes of the line: the places of its items, or of its pairs of items where two CTAs walk a span.
+template <int ROWS> __device__ __forceinline__ int units_of(const KernelParams &p, const TreeSequence &s, int grain) {
+    return s.nodes == 0 ? 0 : (blocks_of<ROWS>(p.t, s) * p.t.kv_heads + p.share - 1) / p.share * pitch_of(tiles_of(s), grain);
 }
 
 // A CTA's way along its span.
 template <int ROWS> struct Walk {
-    int at, end, seq_start, units, span, seq;
+    int at, end, seq_start, units, span, grain, seq;
     TreeSequence s;  // of seq
     __device__ __forceinline__ void next(const KernelParams &p, Segment &g) {
         g.n = 0;
@@ -96,14 +99,15 @@ template <int ROWS> struct Walk {
             if (at >= seq_start + units) {
                 seq_start += units;
                 s = tree_sequence(p.t, ++seq);
-                units = units_of<ROWS>(p, s);
+                units = units_of<ROWS>(p, s, grain);
                 continue;
             }
-            const int tiles = tiles_of(s), blocks = blocks_of<ROWS>(p.t, s);
-            const int pair = (int)((unsigned)(at - seq_start) / (unsigned)tiles), item_start = seq_start + pair * tiles;
+            const int tiles = tiles_of(s), blocks = blocks_of<ROWS>(p.t, s), pitch = pitch_of(tiles, grain);
+            const int pair = (int)((unsigned)(at - seq_start) / (unsigned)pitch), item_start = seq_start + pair * pitch;
             const int lane = p.share == 2 ? (int)blockIdx.x & 1 : 0, item = pair * p.share + lane;
             const int j0 = at - item_start, n = min(tiles - j0, end - at);
-            at += n;
+            at = min(end, item_start + pitch);
+            if (n <= 0) continue;  // behind the item's last tile
             const int kv_head = (int)((unsigned)item / (unsigned)blocks);
             if (kv_head >= p.t.kv_heads) continue;  // an odd number of items: nothing for the second CTA
             g.s = s;
@@ -146,8 +150,6 @@ template <int ROWS, int STAGES> struct Control {
         Segment seg[kSegRing];
         struct {  // before the first is planned
             int sums[16], tops[16];  // of each warp
-            int seq_start, units, seq;
-            TreeSequence s;
         } start;
     };
     uint32_t tmem;
@@ -282,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const 
     // The line's length, then the sequence that this CTA's span starts in: a scan over kThreads sequences at a time, the same once more
     // where there are more.  (What runs once is kept short here and below: instructions that are not in the cache yet come at a
     // tenth of the rate.)
-    int span = 1, begin = 0, end = 0;
+    int span = 1, grain = 1, begin = 0, end = 0;
     {
         int total = 0, before = 0, longest = 0;
         bool counting = true;
@@ -292,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const 
             int units = 0;
             if (base + (int)threadIdx.x < p.t.num_seqs) {
                 mine = tree_sequence(p.t, base + threadIdx.x);
-                units = units_of<ROWS>(p, mine);
+                units = units_of<ROWS>(p, mine, grain);
                 if (mine.code && counting && blockIdx.x == 0) tree_report(p.t, mine.code, base + threadIdx.x);
             }
             int upto = units;
@@ -322,23 +324,35 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const 
                 // Few tiles are not spread over all CTAs: each part costs the end of its item about a third of what a tile takes, so that an
                 // item of t tiles is done first with some sqrt(t / 3) tiles a part (one KV head, 16000 tokens: 90 -> 24 us; 8 heads, 700
                 // tokens: 16.4 -> 14.8).
-                span = max((int)(sqrtf(0.35f * (float)longest) + 0.5f), max(1, (int)((unsigned)(total + spans - 1) / spans)));
-                begin = min(total, span * (int)line);
-                end = min(total, begin + span);
-                if (base > 0) {
+                const int least = (int)(sqrtf(0.35f * (float)longest) + 0.5f), even = (int)((unsigned)(total + spans - 1) / spans);
+                span = max(max(least, 1), even);
+                // A second item in a CTA's span costs it what four tiles take, so items get whole spans where that needs no more than
+                // four tiles more a span (8 heads, 2000 tokens: 21.9 us -> 19; 16000: 36 -> 32), which takes another pass here (1 us) and
+                // is left out where they do anyway.
+                if (p.items > 1 && p.items < (int)spans && (longest % span || total != p.items * longest)) {
+                    const int whole = max(max(least, 1), (int)((unsigned)max(total - p.items, 0) / (spans - p.items)) + 1);
+                    if (whole <= span + 4) span = grain = whole;
+                }
+                begin = span * (int)line;
+                end = begin + span;  // with a grain the line's length is a multiple of it
+                if (grain == 1) {
+                    begin = min(begin, total);
+                    end = min(end, total);
+                }
+                if (base > 0 || grain > 1) {
                     base = -kThreads;
                     continue;
                 }
             }
             upto += before;
-            if (begin < end && begin < upto && begin >= upto - units) {
-                ctl.start.seq = base + threadIdx.x;
-                ctl.start.seq_start = upto - units;
-                ctl.start.units = units;
-                ctl.start.s = mine;
+            if (begin < upto && begin >= upto - units) {
+                ctl.walk = Walk<ROWS>{begin, end, upto - units, units, span, grain, base + (int)threadIdx.x, mine};
             }
             before += pass;
-            if (begin >= end || before > begin) break;
+            if (before > begin || base + kThreads >= p.t.num_seqs) {
+                if (before <= begin) end = begin;  // behind the line's end: nothing to do
+                break;
+            }
         }
     }
     __syncthreads();
@@ -546,10 +560,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const 
             __syncwarp();
         };
         if (plans) {
-            const Walk<ROWS> walk{begin, end, ctl.start.seq_start, ctl.start.units, span, ctl.start.seq, ctl.start.s};
-            __syncwarp();
-            if (lane == 0) ctl.walk = walk;
-            __syncwarp();
 #pragma unroll 1
             for (int k = 0; k < 2 && more; ++k) {
                 plan();
@@ -793,6 +803,8 @@ template <int D, int ROWS> int launch(flat_ctx *ctx, const TreeParams &t) {
     KernelParams p{};
     p.t = t;
     p.share = (int64_t)t.max_nodes * t.group > ROWS ? 2 : 1;
+    const int64_t blocks = ((int64_t)t.max_nodes * t.group + ROWS - 1) / ROWS;
+    p.items = (int)((blocks * t.kv_heads + p.share - 1) / p.share * t.num_seqs);
     p.box_rows = t.page_size % 64 == 0 ? 64 : t.page_size % 32 == 0 ? 32 : 16;
     const uint64_t rows = (uint64_t)t.physical_pages * t.page_size;
     if (int st = make_pool_map(ctx, &p.map_k, t.k, D, rows, t.kv_heads, p.box_rows)) return st;

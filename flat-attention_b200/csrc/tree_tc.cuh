@@ -1,4 +1,4 @@
-// What the tensor-core kernels of the attention of drafted tokens share.
+// Parts of the tensor-core kernel of the attention of drafted tokens: masks, products, TMA, the order of the ring, queries and values.
 #pragma once
 
 #include <cuda.h>

@@ -122,6 +122,17 @@ def test_items_over_many_parts_and_blocks_that_do_not_divide(dtype, Hq, Hkv, D, 
     assert torch.equal(first, t.raw)
 
 
+@pytest.mark.parametrize("Hq,Hkv,n", [(2, 2, 3), (8, 8, 1), (3, 1, 40), (4, 2, 70)])
+def test_items_cut_into_parts_of_every_number(Hq, Hkv, n):
+    """Sequences of 1 to 40 tiles, alone and with others: parts that end with their item and parts that do not."""
+    c = ctx()
+    for tiles in [*range(1, 24), 33, 40]:
+        for lens in ([64 * tiles - n - 1], [64 * tiles, 64 * (41 - tiles) + 1], [64 * tiles - n, 5, 64 * tiles - n, 64 * tiles - n]):
+            lens = [max(x, 0) for x in lens]
+            t = TreeCase(tiles, fa.BF16, Hq, Hkv, 64, 64, lens, [n] + [max(1, n - 2)] * (len(lens) - 1))
+            t.check(t.run(c), t.exact())
+
+
 @pytest.mark.parametrize("dtype,Hq,Hkv,D", [(fa.BF16, 4, 2, 64), (fa.BF16, 8, 1, 128), (fa.F32, 2, 1, 32)])
 @pytest.mark.parametrize("S", [255, 257, 700])
 def test_more_sequences_than_a_block_has_threads(dtype, Hq, Hkv, D, S):
