@@ -243,48 +243,51 @@ template <typename T, int HALVES> __global__ void __launch_bounds__(kThreads) tr
     }
 }
 
-// Joins the chunks of the rows of one sequence's drafted token: LSE = log sum exp(LSE_i), O = sum exp(LSE_i - LSE) O_i, a head a
-// warp.  Lanes take chunks for the weights and dims for the sum, which goes in chunk order.
-template <typename T> __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__ TreeParams p) {
-    __shared__ float w_s[4][kMaxSplits];
+// Joins the chunks of one drafted token's head: LSE = log sum exp(LSE_i), O = sum exp(LSE_i - LSE) O_i.  Threads take chunks for the
+// weights; for the sum four dims each, and groups of threads every so many-th chunk, added up in a fixed order.
+template <typename T> __global__ void __launch_bounds__(kThreads) tree_merge_kernel(const __grid_constant__ TreeParams p) {
+    constexpr int kWarps = kThreads / 32;
+    __shared__ float w[kMaxSplits], top_s[kWarps], sum_s[kWarps];
+    __shared__ float4 o_s[kWarps][32];
     grid_dependency_wait();
     grid_dependency_launch();
-    const int seq = blockIdx.z, node = blockIdx.y, lane = threadIdx.x & 31;
+    const int seq = blockIdx.z, node = blockIdx.y, head = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const TreeSequence s = tree_sequence(p, seq);
     if (node >= s.nodes) return;
     const int parts = max(1, (s.tokens + p.chunk - 1) / p.chunk), D = p.head_dim;
-    const int64_t rows = (int64_t)p.max_q * p.q_heads;
-    float *w = w_s[threadIdx.x >> 5];
-    const int head = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (head >= p.q_heads) return;
-    const int64_t row = (int64_t)(s.first + node) * p.q_heads + head;
+    const int64_t rows = (int64_t)p.max_q * p.q_heads, row = (int64_t)(s.first + node) * p.q_heads + head;
+    auto larger = [](float a, float b) { return b > a || b != b ? b : a; };  // a NaN stays one
     float mx = -INFINITY, sum = 0.f;
-    for (int i = lane; i < parts; i += 32) {
+    for (int i = threadIdx.x; i < parts; i += kThreads) {
         const float x = p.partial_lse[i * rows + row];
         w[i] = x;
-        mx = x > mx || x != x ? x : mx;
+        mx = larger(mx, x);
     }
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) {
-        const float x = __shfl_xor_sync(0xffffffffu, mx, d);
-        mx = x > mx || x != x ? x : mx;  // a NaN stays one
-    }
+    for (int d = 16; d >= 1; d >>= 1) mx = larger(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    if (lane == 0) top_s[warp] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) mx = larger(mx, top_s[i]);
     const float base = mx == -INFINITY ? 0.f : mx;
-    for (int i = lane; i < parts; i += 32) sum += w[i] = expf(w[i] - base);
+    for (int i = threadIdx.x; i < parts; i += kThreads) sum += w[i] = expf(w[i] - base);
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    __syncwarp();
+    if (lane == 0) sum_s[warp] = sum;
+    __syncthreads();
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) sum += sum_s[i];
     const bool empty = sum == 0.f;
     const float inv = empty ? 0.f : 1.0f / sum;
-    // four dims a lane; lanes that are left take every second (fourth, ..) chunk
-    int width = 1;
+    int width = 1;  // threads of a row
     while (width * 4 < D) width *= 2;
-    const int groups = 32 / width, d = lane % width * 4;
+    const int groups = kThreads / width, d = threadIdx.x % width * 4;
     float o[4] = {0.f, 0.f, 0.f, 0.f};
     if (d < D) {
         const bool vec = D % 4 == 0;  // the partial results' rows then are whole groups of four
 #pragma unroll 8
-        for (int i = lane / width; i < parts; i += groups) {
+        for (int i = threadIdx.x / width; i < parts; i += groups) {
             const float4 x = load4<float>(p.partial_o + (i * rows + row) * D + d, vec, D - d);
             const float f = w[i];
             o[0] = fmaf(f, x.x, o[0]);  // a chunk in which the row sees nothing holds zeros
@@ -296,11 +299,19 @@ template <typename T> __global__ void __launch_bounds__(128) tree_merge_kernel(c
     for (int g = 16; g >= width; g /= 2)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += __shfl_xor_sync(0xffffffffu, o[e], g);
-    if (lane < width)
+    o_s[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
+    __syncthreads();
+    if (threadIdx.x < width) {  // 32 threads a row at most
+#pragma unroll
+        for (int i = 1; i < kWarps; ++i) {
+            const float4 x = o_s[i][threadIdx.x];
+            o[0] += x.x, o[1] += x.y, o[2] += x.z, o[3] += x.w;
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (d + e < D) static_cast<T *>(p.o)[row * D + d + e] = from_float<T>(o[e] * inv);
-    if (lane == 0) p.lse[row] = empty ? -INFINITY : base + logf(sum);
+    }
+    if (threadIdx.x == 0) p.lse[row] = empty ? -INFINITY : base + logf(sum);
 }
 
 template <typename T> int launch(flat_ctx *ctx, TreeParams &p) {
@@ -329,7 +340,7 @@ template <typename T> int launch(flat_ctx *ctx, TreeParams &p) {
     }
     ctx->launches += 1;
     if (p.splits > 1) {
-        FLAT_CUDA_OK(ctx, launch_dependent(true, tree_merge_kernel<T>, dim3((unsigned)((p.q_heads + 3) / 4), (unsigned)p.max_nodes, (unsigned)p.num_seqs), 128, 0,
+        FLAT_CUDA_OK(ctx, launch_dependent(true, tree_merge_kernel<T>, dim3((unsigned)p.q_heads, (unsigned)p.max_nodes, (unsigned)p.num_seqs), kThreads, 0,
                                            ctx->stream, p));
         ctx->launches += 1;
     }
