@@ -271,15 +271,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const 
         tma_prefetch_desc(&p.map_k);
         tma_prefetch_desc(&p.map_v);
     }
+    // rows that are not there are zeros, see above
+    for (int i = threadIdx.x; i < 2 * C::kQTile / 16; i += kThreads) reinterpret_cast<uint4 *>(q_s)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async();
+    // TMEM behind the wait: a kernel before this one may still be about to allocate all of it.  The next kernel comes in behind
+    // the barriers below, when this CTA has its own.
+    grid_dependency_wait();
     if (warp == kMmaWarp) {
         tmem_alloc(smem_u32(&ctl.tmem), 512 / kCtasPerSm);
         tmem_relinquish();
     }
-    // rows that are not there are zeros, see above
-    for (int i = threadIdx.x; i < 2 * C::kQTile / 16; i += kThreads) reinterpret_cast<uint4 *>(q_s)[i] = make_uint4(0, 0, 0, 0);
-    fence_proxy_async();
-    grid_dependency_wait();
-    grid_dependency_launch();
 
     // The line's length, then the sequence that this CTA's span starts in: a scan over kThreads sequences at a time, the same once more
     // where there are more.  (What runs once is kept short here and below: instructions that are not in the cache yet come at a
@@ -356,6 +357,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const 
         }
     }
     __syncthreads();
+    grid_dependency_wait();  // long over
+    grid_dependency_launch();
     const uint32_t tmem_base = ctl.tmem;
     auto col_s = [](int b) { return (uint32_t)(D + b * kTok); };  // O in columns 0 .. D - 1
     bool ok = true;
