@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const 
         for (int k = 0;; ++k) {
             const Segment &g = segment(k);
             if (!ok || g.n == 0) break;
-            const int rows = g.rows, n = g.n, j0 = g.j0, len = g.s.len;
+            const int rows = g.rows, n = g.n, j0 = g.j0, all_see = min(g.s.len, g.s.tokens);  // live tokens that are not cut off
             const bool live = row < rows, warp_live = warp * C::kWarpRows < rows;
             const int node = live ? (g.row0 + row) / p.t.group : 0;
             uint32_t own0 = 0, own1 = 0;  // first mask bits
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const 
                     tmem_ld32(tmem_base + lanes + col_s(b) + 32, x + 32);
                     const uint32_t valid = *reinterpret_cast<volatile uint8_t *>(&ctl.valid[count % kValidRing]);  // 16-token groups whose page is in the pool
                     const int t0 = (j0 + i) * kTok;
-                    const bool masked = t0 + kTok > len || valid != 0xf;
+                    const bool masked = t0 + kTok > all_see || valid != 0xf;
                     uint64_t on = ~0ull;
                     if (masked) {
                         on = visible(p.t, g.s, node, t0, own0 | (uint64_t)own1 << 32);
