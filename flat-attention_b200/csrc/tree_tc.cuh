@@ -155,7 +155,10 @@ template <int BOXES, int TOKENS> __device__ __forceinline__ bool clear_values(ui
     return met;
 }
 
-// 8 dims of a query: turned, and written as the sum of two bf16 numbers at `to` and `to` + LO.
+// 8 dims of a query: turned, and written as the sum of two bf16 numbers at `to` and `to` + LO.  The first one is cut off, not rounded, and
+// 2^-30 of the value goes to the second: both then have the value's sign (down to 2^-96), so that their products with a K that is infinite
+// are the same infinity and not its difference.  What is left over is below 2^(e - 7) for a value of 2^e to 2^(e + 1), and bf16 numbers
+// there are 2^(e - 15) apart: the sum is off by 2^-16 of the value at most.
 template <int LO> __device__ __forceinline__ void write_query(uint4 raw, const float2 (&cs)[4], uint8_t *to) {
     const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
     uint32_t hi[4], lo[4];
@@ -163,10 +166,9 @@ template <int LO> __device__ __forceinline__ void write_query(uint4 raw, const f
     for (int e = 0; e < 4; ++e) {
         const float a = __uint_as_float(x[e] << 16), b = __uint_as_float(x[e] & 0xffff0000u);
         const float u = a * cs[e].x - b * cs[e].y, v = a * cs[e].y + b * cs[e].x;
-        const __nv_bfloat162 h2 = __floats2bfloat162_rn(u, v);
-        const float2 f = __bfloat1622float2(h2);
-        hi[e] = *reinterpret_cast<const uint32_t *>(&h2);
-        lo[e] = pack_bf16(u - f.x, v - f.y);
+        const uint32_t ub = __float_as_uint(u), vb = __float_as_uint(v);
+        hi[e] = __byte_perm(ub, vb, 0x7632);  // the upper halves
+        lo[e] = pack_bf16(fmaf(u, 0x1p-30f, u - __uint_as_float(ub & 0xffff0000u)), fmaf(v, 0x1p-30f, v - __uint_as_float(vb & 0xffff0000u)));
     }
     *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     *reinterpret_cast<uint4 *>(to + LO) = make_uint4(lo[0], lo[1], lo[2], lo[3]);

@@ -1,10 +1,10 @@
-"""The serving calls at the limits of what a batch may hold: tokens cut off by a bound or by the pages held.  Models, tolerances
-and helpers are those of test_gpu_paged_serving."""
+"""The serving calls at the limits of what a batch may hold: tokens cut off by a bound or by the pages held, infinite K in tokens
+that are seen.  Models, tolerances and helpers are those of test_gpu_paged_serving."""
 import numpy as np
 import pytest
 
 from tests.gpu_util import ctx, fa
-from tests.test_gpu_paged_serving import TreeCase
+from tests.test_gpu_paged_serving import TreeCase, turned64
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +28,33 @@ def test_live_tokens_that_are_cut_off_do_not_count(dtype, Hq, Hkv, D, lens, node
         t.held = np.array(held, np.int32)
     got = t.run(ctx(), max_context=most, status=35)
     t.check(got, t.exact(drop=[(s, n, a + b) for s, (n, a, b) in enumerate(zip(left, lens, nodes)) if n < a + b]))
+
+
+# ---- K that is infinite in a token that is seen ------------------------------------------------------
+
+@pytest.mark.parametrize("shape", [(fa.BF16, 8, 2, 128, 16), (fa.BF16, 8, 2, 64, 16), (fa.BF16, 4, 2, 96, 16), (fa.F32, 4, 2, 64, 16)], ids=str)
+@pytest.mark.parametrize("lens,nodes", [([90], [9]), ([300, 20], [40, 3]), ([5000], [3])], ids=str)
+@pytest.mark.parametrize("exact_queries", [False, True])
+def test_an_infinite_k_counts_for_nothing_where_the_score_falls_and_makes_the_row_nan_where_it_rises(shape, lens, nodes, exact_queries):
+    """Products with an infinity have the query's sign: a score of -inf has weight 0, one of +inf leaves no weights.  exact_queries:
+    turned and scaled queries that are bf16 numbers, of which nothing is left over for a second summand."""
+    t = TreeCase(sum(lens) + shape[3], *shape, lens, nodes)
+    cfg, scale = fa.config(True), None
+    if exact_queries:
+        f = np.float32
+        scale = next(x for x in (f(1) / f(1.4426950408889634) + f(i) * f(2.0 ** -24) for i in (0, 1, -1, 2, -2)) if f(x) * f(1.4426950408889634) == f(1))
+        cfg, scale = fa.config(True, float(scale)), float(scale)
+        t.positions[:] = 0
+    D, G = t.D, t.Hq // t.Hkv
+    at = t.row(0, lens[0] // 2)
+    want = t.exact(scale=scale, drop=[(0, lens[0] // 2, lens[0] // 2 + 1)])
+    q = turned64(t.q[:t.T].double().numpy(), t.positions[:t.T], D).reshape(t.T, t.Hq, D)[:nodes[0]]
+    t.k[at, 6], t.k[at, D + 7] = float("inf"), -float("inf")  # head 0, dim 6; head 1, dim 7
+    signs = np.concatenate([q[:, :G, 6], -q[:, G:2 * G, 7]], 1)
+    assert (np.abs(signs) > 2.0 ** -20).all() and (signs < 0).any() and (signs > 0).any()
+    o, lse = t.run(ctx(), cfg=cfg)
+    rises = np.zeros((t.T, t.Hq), bool)
+    rises[:nodes[0], :2 * G] = signs > 0
+    assert np.isnan(o[rises]).all() and np.isnan(lse[rises]).all()
+    o[rises], lse[rises] = want[0][rises], want[1][rises]
+    t.check((o, lse), want)
