@@ -65,6 +65,18 @@ int ensure_paged_scratch(flat_ctx *ctx) {
 
 namespace {
 
+// Work goes to the context's device whatever device is current.
+struct DeviceGuard {
+    int before = -1;
+    explicit DeviceGuard(const flat_ctx *ctx) {
+        int current = -1;
+        if (cudaGetDevice(&current) == cudaSuccess && current != ctx->device && cudaSetDevice(ctx->device) == cudaSuccess) before = current;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
 struct Dims {
     uint64_t q_elements, kv_elements, lse_elements;
 };
@@ -771,24 +783,27 @@ int32_t flat_ctx_device_status(flat_ctx *ctx) {
     DeviceStatus h{};
     FLAT_CUDA_OK(ctx, cudaStreamSynchronize(ctx->stream));
     FLAT_CUDA_OK(ctx, cudaMemcpy(&h, ctx->dev_status, sizeof h, cudaMemcpyDeviceToHost));
-    if (h.code != 0) {
-        if (h.code == FLAT_ERR_PAGE_OUT_OF_RANGE)
-            fail(ctx, h.code, "a page-table entry of sequence %d lies outside the physical pool; its tokens were masked", h.where);
-        else if (h.code == FLAT_ERR_NON_FINITE_INPUT)
-            fail(ctx, h.code, "a device-side input scan found a non-finite value (tensor %d)", h.where);
-        else if (h.code == FLAT_ERR_CAPACITY_EXCEEDED)
-            fail(ctx, h.code, "the free pages do not hold the new tokens of sequence %d", h.where);
-        else if (h.code == FLAT_ERR_CAPACITY_OVERFLOW)
-            fail(ctx, h.code, "the count of free pages leaves the pool (sequence %d)", h.where);
-        else if (h.code == FLAT_ERR_INVALID_CACHE_LENGTH || h.code == FLAT_ERR_LENGTH_MISMATCH)
-            fail(ctx, h.code, "lengths of sequence %d do not fit its pages or the call's bounds; it was left out", h.where);
+    const int code = (int)(h.word >> 32), where = (int)(uint32_t)h.word;
+    if (code != 0) {
+        const DeviceGuard guard(ctx);
+        if (code == FLAT_ERR_PAGE_OUT_OF_RANGE)
+            fail(ctx, code, "a page-table entry of sequence %d lies outside the physical pool; its tokens were masked", where);
+        else if (code == FLAT_ERR_NON_FINITE_INPUT)
+            fail(ctx, code, "a device-side input scan found a non-finite value (tensor %d)", where);
+        else if (code == FLAT_ERR_CAPACITY_EXCEEDED)
+            fail(ctx, code, "the free pages do not hold the new tokens of sequence %d", where);
+        else if (code == FLAT_ERR_CAPACITY_OVERFLOW)
+            fail(ctx, code, "the count of free pages leaves the pool (sequence %d)", where);
+        else if (code == FLAT_ERR_INVALID_CACHE_LENGTH || code == FLAT_ERR_LENGTH_MISMATCH)
+            fail(ctx, code, "lengths of sequence %d do not fit its pages or the call's bounds; it was left out", where);
         else
-            fail(ctx, h.code, "device wait expired at site %d", h.where);
-        if (h.code == FLAT_ERR_DEVICE_WAIT_TIMEOUT && ctx->paged_scratch)  // a kernel that gave up has not counted to the end
-            cudaMemset(paged_tickets(ctx), 0, (kPagedTickets + 1) * sizeof(unsigned));
-        cudaMemset(ctx->dev_status, 0, sizeof(DeviceStatus));
+            fail(ctx, code, "device wait expired at site %d", where);
+        if (code == FLAT_ERR_DEVICE_WAIT_TIMEOUT && ctx->paged_scratch)  // a kernel that gave up has not counted to the end
+            FLAT_CUDA_OK(ctx, cudaMemsetAsync(paged_tickets(ctx), 0, (kPagedTickets + 1) * sizeof(unsigned), ctx->stream));
+        FLAT_CUDA_OK(ctx, cudaMemsetAsync(ctx->dev_status, 0, sizeof(DeviceStatus), ctx->stream));
+        FLAT_CUDA_OK(ctx, cudaStreamSynchronize(ctx->stream));  // whatever stream the next call is on, it meets them cleared
     }
-    return h.code;
+    return code;
 }
 
 int32_t flat_ctx_set_kernel_timing(flat_ctx *ctx, int32_t enabled) {
@@ -1783,18 +1798,6 @@ int32_t flat_splitkv_merge(flat_ctx *ctx, int32_t dtype, uint64_t parts, uint64_
 }  // extern "C"
 
 namespace {
-
-// Launches go to the context's device whatever device is current.
-struct DeviceGuard {
-    int before = -1;
-    explicit DeviceGuard(const flat_ctx *ctx) {
-        int current = -1;
-        if (cudaGetDevice(&current) == cudaSuccess && current != ctx->device && cudaSetDevice(ctx->device) == cudaSuccess) before = current;
-    }
-    ~DeviceGuard() {
-        if (before >= 0) cudaSetDevice(before);
-    }
-};
 
 int check_ints(flat_ctx *ctx, const char *name, const int32_t *p) {
     if (!p) return fail(ctx, FLAT_ERR_NULL_POINTER, "%s is null", name);

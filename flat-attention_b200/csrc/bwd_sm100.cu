@@ -112,10 +112,7 @@ __device__ __forceinline__ void bulk_copy_s2g(void *dst, uint32_t src, uint32_t 
 }
 
 __device__ __forceinline__ void timeout(const BwdKernelParams &p, int where) {
-    if (p.status) {
-        p.status->code = FLAT_ERR_DEVICE_WAIT_TIMEOUT;
-        p.status->where = where;
-    }
+    if (p.status) report_status(p.status, FLAT_ERR_DEVICE_WAIT_TIMEOUT, where);
 }
 
 // KV-stationary kernel: stationary (K, V), streamed (Q_i, dO_i), outputs dV (out0) and dK (out1).

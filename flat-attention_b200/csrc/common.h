@@ -21,10 +21,10 @@ constexpr int kMaxHeadDim = 128;  // WGSL_MAX_HEAD_DIM, src/lib.rs:60
 constexpr uint64_t kShortPartialBytes = 32ull << 20;  // 508 parts of 32 heads at D = 128
 constexpr uint64_t kF32TableBytes = 16ull << 20;  // 32768 positions at head_dim 128
 
-// Device status word written by bounded waits.
+// Status word of a context, written by kernels and 0 where there is nothing to report: a FLAT_ERR_* code in the upper half, in the lower one
+// which wait gave up (a tag of the kernel) or which sequence or entry of the call is meant.
 struct DeviceStatus {
-    int code;    // FLAT_OK or FLAT_ERR_DEVICE_WAIT_TIMEOUT
-    int where;   // which wait gave up (kernel-specific tag)
+    unsigned long long word;
 };
 
 }  // namespace flat
@@ -167,6 +167,11 @@ inline bool may_overlap_previous(flat_ctx *ctx) {
 #ifdef __CUDACC__
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// The largest word stays, whichever comes last: a code and its place belong together, what is named does not depend on the order of the
+// blocks, and a wait that gave up, whose code is the largest that a kernel reports, is not hidden by a bad page.
+__device__ __forceinline__ void report_status(DeviceStatus *status, int code, int where) {
+    atomicMax(&status->word, (unsigned long long)(unsigned)code << 32 | (unsigned)where);
+}
 #endif
 
 // ---- forward ---------------------------------------------------------------------------------

@@ -136,10 +136,7 @@ __global__ void __launch_bounds__(256) decode_kernel(const __grid_constant__ Dec
                     // an entry outside the pool is never dereferenced: the token is masked and the call is flagged
                     if ((unsigned)page >= (unsigned)p.physical_pages) {
                         ok[u] = false;
-                        if (p.status) {
-                            p.status->code = FLAT_ERR_PAGE_OUT_OF_RANGE;
-                            p.status->where = seq;
-                        }
+                        if (p.status) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, seq);
                     }
                     row = (int64_t)page * p.page_size + t % p.page_size;
                 } else {

@@ -134,10 +134,7 @@ __device__ __forceinline__ int64_t tile_row(const DecodeParams &p, const Table &
     const int page = table.page(p, seq, t0 / p.page_size);
     // an entry outside the pool is never dereferenced: the tile is skipped and the call is flagged
     if ((unsigned)page >= (unsigned)p.physical_pages) {
-        if ((threadIdx.x & 31) == 0 && p.status) {
-            p.status->code = FLAT_ERR_PAGE_OUT_OF_RANGE;
-            p.status->where = seq;
-        }
+        if ((threadIdx.x & 31) == 0 && p.status) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, seq);
         return -1;
     }
     return (int64_t)page * p.page_size + t0 % p.page_size;

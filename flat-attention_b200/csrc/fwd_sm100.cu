@@ -213,10 +213,7 @@ template <int D, bool CONVK> struct Cfg {
 };
 
 __device__ __forceinline__ void record_timeout(const KernelParams &p, int where) {
-    if (p.status) {
-        p.status->code = FLAT_ERR_DEVICE_WAIT_TIMEOUT;
-        p.status->where = where;
-    }
+    if (p.status) report_status(p.status, FLAT_ERR_DEVICE_WAIT_TIMEOUT, where);
 }
 
 // One unit of work: 256 consecutive query rows of one (batch, q_head), over all visible KV tiles or, for a split

@@ -67,11 +67,6 @@ __device__ __forceinline__ void block_scan2(int64_t &x, int64_t &y, int64_t &tot
     total_y = __shfl_sync(0xffffffffu, b, 31);
 }
 
-__device__ __forceinline__ void flag(DeviceStatus *status, int code, int where) {
-    status->code = code;
-    status->where = where;
-}
-
 // The sequence that entry i of a packed list belongs to: the last one that starts at or before i.
 __device__ __forceinline__ int sequence_of(const int32_t *offsets, int num_seqs, int i) {
     int lo = 0, hi = num_seqs;
@@ -100,7 +95,7 @@ __device__ __forceinline__ int64_t most_tokens(const PagedBatchParams &p) {
 __device__ __forceinline__ void reserve_scan(const PagedBatchParams &p) {
     __shared__ int64_t warp_sums[kScanThreads / 32];
     const int f = clamped_free_count(p);
-    if (threadIdx.x == 0 && f != *p.free_count) flag(p.status, FLAT_ERR_CAPACITY_OVERFLOW, -1);
+    if (threadIdx.x == 0 && f != *p.free_count) report_status(p.status, FLAT_ERR_CAPACITY_OVERFLOW, -1);
     int64_t tokens = 0, pages = 0;  // of the sequences before this pass
     int64_t taken = 0;              // pages that are really given out
     const int64_t most = most_tokens(p);
@@ -126,7 +121,7 @@ __device__ __forceinline__ void reserve_scan(const PagedBatchParams &p) {
             p.offsets[s] = (int)min(upto - N, (int64_t)p.max_tokens);
             p.page_counts_out[s] = (int)(granted ? H + need : H);
             if (p.context_lens_out) p.context_lens_out[s] = (int)(granted ? L + N : L);
-            if (!granted) flag(p.status, valid ? FLAT_ERR_CAPACITY_EXCEEDED : FLAT_ERR_INVALID_CACHE_LENGTH, s);
+            if (!granted) report_status(p.status, valid ? FLAT_ERR_CAPACITY_EXCEEDED : FLAT_ERR_INVALID_CACHE_LENGTH, s);
         }
     }
     if (threadIdx.x == 0) {
@@ -160,7 +155,7 @@ __device__ __forceinline__ NewToken reserve_look(const PagedBatchParams &p, cons
 }
 __device__ __forceinline__ int reserve_enter(const PagedBatchParams &p, NewToken x) {  // the token's slot
     if (x.seq >= 0 && (unsigned)x.page >= (unsigned)p.physical_pages) {
-        flag(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, x.seq);
+        report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, x.seq);
         x.page = -1;
     }
     if (x.entry >= 0) p.page_tables[x.entry] = x.page;
@@ -170,7 +165,7 @@ __device__ __forceinline__ int reserve_enter(const PagedBatchParams &p, NewToken
 __device__ __forceinline__ void release_scan(const PagedBatchParams &p) {
     __shared__ int64_t warp_sums[kScanThreads / 32];
     const int f = clamped_free_count(p);
-    if (threadIdx.x == 0 && f != *p.free_count) flag(p.status, FLAT_ERR_CAPACITY_OVERFLOW, -1);
+    if (threadIdx.x == 0 && f != *p.free_count) report_status(p.status, FLAT_ERR_CAPACITY_OVERFLOW, -1);
     const int64_t room = p.physical_pages - f;
     int64_t pages = 0;
     for (int base = 0; base < p.num_seqs; base += kScanThreads) {
@@ -187,8 +182,8 @@ __device__ __forceinline__ void release_scan(const PagedBatchParams &p) {
             p.plan[s] = make_int4(0, (int)H, (int)left, 0);
             p.plan_offsets[s] = (int)min(upto - gone, room);
             p.page_counts_out[s] = (int)left;
-            if (!valid) flag(p.status, FLAT_ERR_INVALID_CACHE_LENGTH, s);
-            else if (upto > room) flag(p.status, FLAT_ERR_CAPACITY_OVERFLOW, s);
+            if (!valid) report_status(p.status, FLAT_ERR_INVALID_CACHE_LENGTH, s);
+            else if (upto > room) report_status(p.status, FLAT_ERR_CAPACITY_OVERFLOW, s);
         }
     }
     if (threadIdx.x == 0) {
@@ -201,7 +196,7 @@ __device__ __forceinline__ void release_scan(const PagedBatchParams &p) {
 __device__ __forceinline__ void release_page(const PagedBatchParams &p, int i, int f) {
     const int s = sequence_of(p.plan_offsets, p.num_seqs, i);
     const int page = p.page_tables[(int64_t)s * p.max_pages + p.plan[s].y - 1 - (i - p.plan_offsets[s])];
-    if ((unsigned)page >= (unsigned)p.physical_pages) flag(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, s);
+    if ((unsigned)page >= (unsigned)p.physical_pages) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, s);
     p.free_pages[f + i] = page;
 }
 
@@ -339,7 +334,7 @@ template <bool RELEASE> __global__ void __launch_bounds__(kScanThreads) paged_ba
 #pragma unroll
             for (int u = 0; u < kItems; ++u) {
                 if (u >= n) break;
-                if ((unsigned)page[u] >= (unsigned)p.physical_pages) flag(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, seq[u]);
+                if ((unsigned)page[u] >= (unsigned)p.physical_pages) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, seq[u]);
                 p.free_pages[f + i0 + u] = page[u];
             }
         } else {
@@ -377,12 +372,12 @@ template <bool RELEASE> __global__ void __launch_bounds__(kScanThreads) paged_ba
                 p.offsets[s] = starts_s[s];
                 if (p.context_lens_out) p.context_lens_out[s] = flags[i] == FLAT_OK ? L[i] + A[i] : L[i];
             }
-            if (flags[i] != FLAT_OK) flag(p.status, flags[i], s);
+            if (flags[i] != FLAT_OK) report_status(p.status, flags[i], s);
         }
         if (threadIdx.x == 0) {
             if (!RELEASE) p.offsets[p.num_seqs] = (int)total;
             *p.free_count_out = RELEASE ? f + (int)total : f - taken_s;
-            if (f != given) flag(p.status, FLAT_ERR_CAPACITY_OVERFLOW, -1);
+            if (f != given) report_status(p.status, FLAT_ERR_CAPACITY_OVERFLOW, -1);
         }
     }
 }

@@ -12,11 +12,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxBlockTokens = 8;
 
-__device__ __forceinline__ void flag(DeviceStatus *status, int code, int where) {
-    status->code = code;
-    status->where = where;
-}
-
 __device__ __forceinline__ uint4 load16(const void *p) {
     uint4 r;
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
@@ -62,7 +57,7 @@ __global__ void __launch_bounds__(kThreads) paged_write_kernel(const __grid_cons
     const int n = (int)min((int64_t)p.block_tokens, p.tokens - first);
     if (threadIdx.x < n) {
         const int slot = p.slots[first + threadIdx.x];
-        if (slot >= p.pool_rows) flag(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, (int)(first + threadIdx.x));
+        if (slot >= p.pool_rows) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, (int)(first + threadIdx.x));
         row_s[threadIdx.x] = slot < p.pool_rows ? slot : -1;
     }
     const int total = n * vecs;
@@ -121,7 +116,7 @@ __global__ void __launch_bounds__(kThreads) paged_write_pairs_kernel(const __gri
         const int64_t row = p.slots[t];
         if (row < 0) continue;
         if (row >= p.pool_rows) {
-            if (e == 0) flag(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, (int)t);
+            if (e == 0) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, (int)t);
             continue;
         }
         const bool two = e + 1 < p.row_elems;
@@ -177,11 +172,11 @@ template <typename V> __global__ void __launch_bounds__(kThreads) paged_accept_k
         for (int base = (max(take, 1) - 1) / kSteps * kSteps; base >= 0; base -= kSteps) look(base);
     __syncthreads();
     const bool bad = bad_s != 0;
-    if (threadIdx.x == 0) {  // context_lens_out may be context_lens: every thread has read the length
-        p.context_lens_out[seq] = bad ? len : len + take;
-        if (bad) flag(p.status, FLAT_ERR_LENGTH_MISMATCH, seq);
+    if (threadIdx.x == 0) p.context_lens_out[seq] = bad ? len : len + take;  // may be context_lens: every thread has read the length
+    if (bad) {
+        if (threadIdx.x == 0) report_status(p.status, FLAT_ERR_LENGTH_MISMATCH, seq);
+        return;
     }
-    if (bad) return;
     for (int base = 0; base < take; base += kSteps) {
         if (base > 0) {
             __syncthreads();

@@ -92,10 +92,7 @@ __global__ void __launch_bounds__(kXchgThreads) peer_exchange_merge_kernel(const
         while (ld_acquire_sys(flag) != epoch) {
             if (clock64() - start > kXchgWaitCycles) {
                 give_up = 1;
-                if (p.status) {
-                    p.status->code = FLAT_ERR_DEVICE_WAIT_TIMEOUT;
-                    p.status->where = 500 + tid;
-                }
+                if (p.status) report_status(p.status, FLAT_ERR_DEVICE_WAIT_TIMEOUT, 500 + tid);
                 break;
             }
             __nanosleep(40);

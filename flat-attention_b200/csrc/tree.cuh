@@ -29,11 +29,6 @@ __device__ __forceinline__ TreeSequence tree_sequence(const TreeParams &p, int s
     if (s.tokens < want) s.code = FLAT_ERR_PAGE_OUT_OF_RANGE;
     return s;
 }
-__device__ __forceinline__ void tree_report(const TreeParams &p, int code, int seq) {
-    p.status->code = code;
-    p.status->where = seq;
-}
-
 // Whether drafted token `node` sees drafted token j of its sequence.
 __device__ __forceinline__ bool tree_sees(const TreeParams &p, const TreeSequence &s, int node, int j) {
     if (!p.mask) return !p.causal || j <= node;

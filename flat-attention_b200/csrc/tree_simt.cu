@@ -43,7 +43,7 @@ template <> __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bf
 
 __device__ __forceinline__ TreeSequence span_of(const TreeParams &p, int seq) {
     const TreeSequence s = tree_sequence(p, seq);
-    if (s.code && threadIdx.x == 0) tree_report(p, s.code, seq);
+    if (s.code && threadIdx.x == 0) report_status(p.status, s.code, seq);
     return s;
 }
 
@@ -84,8 +84,7 @@ template <typename T, int HALVES> __global__ void __launch_bounds__(kThreads) tr
                 if ((unsigned)page < (unsigned)p.physical_pages) {
                     at[i] = (((int64_t)page * p.page_size + t - logical * p.page_size) * p.kv_heads + kv_head) * D;
                 } else if ((tid & 15) == 0) {  // never read: its tokens are left out and the call is flagged
-                    p.status->code = FLAT_ERR_PAGE_OUT_OF_RANGE;
-                    p.status->where = seq;
+                    report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, seq);
                 }
             }
         }

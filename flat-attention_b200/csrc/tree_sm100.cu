@@ -131,8 +131,7 @@ template <int ROWS> struct Walk {
 };
 
 __device__ __forceinline__ void record_timeout(const KernelParams &p, int where) {
-    p.t.status->code = FLAT_ERR_DEVICE_WAIT_TIMEOUT;
-    p.t.status->where = where;
+    report_status(p.t.status, FLAT_ERR_DEVICE_WAIT_TIMEOUT, where);
 }
 
 // Whether tile j of the segment's item holds drafted tokens or is its last: its V tile is gone over before it is used.  (Every
@@ -296,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const 
             if (base + (int)threadIdx.x < p.t.num_seqs) {
                 mine = tree_sequence(p.t, base + threadIdx.x);
                 units = units_of<ROWS>(p, mine, grain);
-                if (mine.code && counting && blockIdx.x == 0) tree_report(p.t, mine.code, base + threadIdx.x);
+                if (mine.code && counting && blockIdx.x == 0) report_status(p.t.status, mine.code, base + threadIdx.x);
             }
             int upto = units;
 #pragma unroll
@@ -667,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const 
                     if (all) {
                         for (int e = 0; e < 4; ++e)
                             if ((all >> (e * 16 / p.box_rows)) & 1 && e * 16 / p.box_rows < boxes) valid &= ~(1u << e);
-                        if (lane == 0 && valid != 0xf) tree_report(p.t, FLAT_ERR_PAGE_OUT_OF_RANGE, g.seq);
+                        if (lane == 0 && valid != 0xf) report_status(p.t.status, FLAT_ERR_PAGE_OUT_OF_RANGE, g.seq);
                     }
                     if (lane == 0) ctl.valid[count % kValidRing] = (uint8_t)valid;
                 }

@@ -215,7 +215,9 @@ int32_t flat_ctx_reserve_rope_tables(flat_ctx *ctx, uint64_t rows, uint64_t head
 uint64_t flat_ctx_launch_count(const flat_ctx *ctx);
 /* Reads the device status word written by kernels: FLAT_OK, FLAT_ERR_DEVICE_WAIT_TIMEOUT (a
  * bounded wait gave up) or FLAT_ERR_PAGE_OUT_OF_RANGE (a decode kernel met a page-table entry
- * outside the pool and masked its tokens); synchronises the stream and clears the word. */
+ * outside the pool and masked its tokens), or what the calls on device-resident batches below name; of several faults the
+ * largest code with its largest place, so that a wait that gave up is never hidden.  Synchronises the stream, clears the word
+ * and, after a wait that gave up, the counters that its kernel may have left half way. */
 int32_t flat_ctx_device_status(flat_ctx *ctx);
 
 /* Kernel timing for benchmarks (the reference benches time encode+submit+poll on the host,

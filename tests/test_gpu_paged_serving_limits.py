@@ -1,10 +1,12 @@
 """The serving calls at the limits of what a batch may hold: tokens cut off by a bound or by the pages held, infinite K in tokens
-that are seen.  Models, tolerances and helpers are those of test_gpu_paged_serving."""
+that are seen, faults reported next to one another.  Models, tolerances and helpers are those of test_gpu_paged_serving."""
 import numpy as np
 import pytest
+import torch
 
 from tests.gpu_util import ctx, fa
-from tests.test_gpu_paged_serving import TreeCase, turned64
+from tests.test_gpu_decode_cache import _one_sequence_slice
+from tests.test_gpu_paged_serving import THETA, TreeCase, clean, i32, turned64
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +60,45 @@ def test_an_infinite_k_counts_for_nothing_where_the_score_falls_and_makes_the_ro
     assert np.isnan(o[rises]).all() and np.isnan(lse[rises]).all()
     o[rises], lse[rises] = want[0][rises], want[1][rises]
     t.check((o, lse), want)
+
+
+# ---- faults reported next to one another -------------------------------------------------------------
+
+def write_behind_the_pool(c, bad, tokens=2000):
+    """A row write whose tokens `bad` name slots behind the pool."""
+    src, pool = torch.ones(tokens, 64, device="cuda", dtype=torch.bfloat16), torch.zeros(tokens, 64, device="cuda", dtype=torch.bfloat16)
+    slots = np.arange(tokens)
+    slots[bad] = tokens + 5
+    c.paged_kv_write(1, 64, i32(slots), None, THETA, src, src, pool, pool.clone())
+
+
+def test_a_wait_that_gave_up_is_not_hidden_by_what_is_reported_behind_it():
+    """The exchange waits for a rank that does not exist and gives up after about a second (a bounded wait); a bad slot is reported
+    behind it, before the status is read.  What gave up may have left counters half way: the status has to say so."""
+    c = fa.Context(0)
+    t = TreeCase(55, fa.BF16, 8, 2, 128, 16, [900, 40], [9, 3])
+    want = t.exact()
+    t.check(t.run(c), want)
+    args, Hq, D = _one_sequence_slice(16 * 40)
+    x = fa.SplitKvPeerExchange(c, 0, 2, Hq, D)
+    try:
+        x.connect(x.handle() * 2)
+        out = c.create_decode_output_buffer(fa.BF16, 1, Hq, D)
+        c.splitkv_decode_peer(x, fa.BF16, *args, out)
+        write_behind_the_pool(c, [3])
+        c.synchronize()
+        assert fa.STATUS[c.device_status()] == "DeviceWaitTimeout"
+        assert c.device_status() == 0
+    finally:
+        x.close()
+    t.check(t.run(c), want)
+    clean(c)
+    c.close()
+
+
+def test_what_the_status_names_does_not_depend_on_the_order_of_the_blocks():
+    c = ctx()
+    for _ in range(20):
+        write_behind_the_pool(c, [3, 700, 1400, 1999])
+        assert c.device_status() == 35
+        assert "1999" in fa.lib().flat_last_error_detail(c.h).decode()
