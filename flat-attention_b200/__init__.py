@@ -686,26 +686,38 @@ def _whole(x) -> Buffer:
 
 class PagedBatch:
     """A batch of sequences over one pool of pages, its page tables, lengths and free pages in device memory (flat_paged_batch).
-    Tensors that are not given start empty: no sequence holds a page, and all pages of the pool are free, the lowest on top."""
+    Tensors that are not given start empty: no sequence holds a page, and all pages of the pool are free, the lowest on top.
+
+    The five tensors may be replaced (`batch.page_counts = counts_out` after a call out of place): later calls use the new one, a
+    captured graph keeps the old one's address.  The sizes are fixed."""
+
+    SIZES = ("num_seqs", "page_size", "physical_pages", "max_pages_per_seq")
+    TENSORS = ("page_tables", "page_counts", "context_lens", "free_pages", "free_count")
 
     def __init__(self, num_seqs: int, page_size: int, physical_pages: int, max_pages_per_seq: int, page_tables=None, page_counts=None,
                  context_lens=None, free_pages=None, free_count=None, device: int = 0, dtype: int = BF16):
         torch = _torch()
         on = dict(dtype=torch.int32, device=f"cuda:{device}")
-        self.num_seqs, self.page_size, self.physical_pages, self.max_pages_per_seq = num_seqs, page_size, physical_pages, max_pages_per_seq
+        self.raw = PagedBatchRaw(num_seqs, page_size, physical_pages, max_pages_per_seq)
+        self.ref = C.byref(self.raw)
         self.dtype = dtype  # of the pool, where calls are given flat_buffer views instead of tensors
+        self.num_seqs, self.page_size, self.physical_pages, self.max_pages_per_seq = num_seqs, page_size, physical_pages, max_pages_per_seq
         self.page_tables = torch.full((num_seqs, max_pages_per_seq), -1, **on) if page_tables is None else page_tables
         self.page_counts = torch.zeros(num_seqs, **on) if page_counts is None else page_counts
         self.context_lens = torch.zeros(num_seqs, **on) if context_lens is None else context_lens
         self.free_pages = torch.arange(physical_pages - 1, -1, -1, **on) if free_pages is None else free_pages
         self.free_count = torch.full((1,), physical_pages, **on) if free_count is None else free_count
-        _ints(num_seqs * max_pages_per_seq, page_tables=self.page_tables)
-        _ints(num_seqs, page_counts=self.page_counts, context_lens=self.context_lens)
-        _ints(physical_pages, free_pages=self.free_pages)
-        _ints(1, free_count=self.free_count)
-        self.raw = PagedBatchRaw(num_seqs, page_size, physical_pages, max_pages_per_seq, *(
-            t.data_ptr() for t in (self.page_tables, self.page_counts, self.context_lens, self.free_pages, self.free_count)))
-        self.ref = C.byref(self.raw)
+
+    def __setattr__(self, name, value):
+        if name in self.TENSORS:  # the calls go by the address, so the two are renewed together
+            need = {"page_tables": self.num_seqs * self.max_pages_per_seq, "free_pages": self.physical_pages, "free_count": 1}.get(name, self.num_seqs)
+            if value is None:
+                raise FlatAttentionError(27, f"{name} is None")
+            _ints(need, **{name: value})
+            setattr(self.raw, name, value.data_ptr())
+        elif name in self.SIZES and name in self.__dict__:
+            raise AttributeError(f"{name} of a PagedBatch is fixed")
+        object.__setattr__(self, name, value)
 
 
 # ---- PagedKvTable (src/paged_kv.rs:75-188) -----------------------------------------------------

@@ -1,5 +1,5 @@
 """The serving calls at the limits of what a batch may hold: tokens cut off by a bound or by the pages held, infinite K in tokens
-that are seen, faults reported next to one another.  Models, tolerances and helpers are those of test_gpu_paged_serving."""
+that are seen, faults reported next to one another, results that take the place of a batch's tensors.  Models, tolerances and helpers are those of test_gpu_paged_serving."""
 import numpy as np
 import pytest
 import torch
@@ -102,3 +102,29 @@ def test_what_the_status_names_does_not_depend_on_the_order_of_the_blocks():
         write_behind_the_pool(c, [3, 700, 1400, 1999])
         assert c.device_status() == 35
         assert "1999" in fa.lib().flat_last_error_detail(c.h).decode()
+
+
+# ---- results of a call out of place that take the place of the batch's tensors -----------------------
+
+def test_counts_written_out_of_place_are_used_once_they_are_the_batch_s():
+    c = ctx()
+    new, keep = i32([5, 0, 17]), i32([3, 0, 20])
+    batches = [fa.PagedBatch(3, 4, 20, 8) for _ in range(2)]
+    rows = [[torch.zeros(n, dtype=torch.int32, device="cuda") for n in (4, 22, 22)] for _ in batches]
+    for step in range(2):
+        a, b = batches
+        c.paged_batch_reserve(a, new, 22, *rows[0], context_lens_out=a.context_lens)
+        counts, free, lens = torch.empty_like(b.page_counts), torch.empty_like(b.free_count), torch.empty_like(b.context_lens)
+        c.paged_batch_reserve(b, new, 22, *rows[1], page_counts_out=counts, free_count_out=free, context_lens_out=lens)
+        b.page_counts, b.free_count, b.context_lens = counts, free, lens
+        for x, y in zip(*rows):
+            assert torch.equal(x, y), step
+        c.paged_batch_release(a, keep)
+        counts, free = torch.empty_like(b.page_counts), torch.empty_like(b.free_count)
+        c.paged_batch_release(b, keep, counts, free)
+        b.page_counts, b.free_count = counts, free
+        for batch in batches:
+            batch.context_lens = keep.clone()
+        assert c.device_status() == (31 if step else 0)  # 20 + 17 tokens are more than the 8 pages of a row of the table
+        assert a.page_counts.tolist() == b.page_counts.tolist() == [1, 0, 5] and a.free_count.item() == b.free_count.item() == 14
+        assert torch.equal(a.free_pages[:14], b.free_pages[:14])
