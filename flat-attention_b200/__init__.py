@@ -481,28 +481,33 @@ class Context:
                                             C.c_uint64(head_dim), buf(partial_o), buf(partial_lse), buf(out)))
 
     # ---- batches whose lengths and page tables stay on the device ----
+    def _device_of(self, batch: "PagedBatch") -> int:
+        if batch.device != self.device:
+            raise FlatAttentionError(29, f"the batch is on cuda:{batch.device}, the context on cuda:{self.device}")
+        return self.device
+
     def paged_batch_reserve(self, batch: "PagedBatch", new_lens, max_new_tokens: int, new_offsets, slot_map, positions, depths=None,
                             page_counts_out=None, free_count_out=None, context_lens_out=None):
         """Pages and slots for new_lens[s] tokens behind each sequence's live ones (flat_paged_batch_reserve); outputs None: in place,
         context_lens_out None: not written."""
-        S, T = batch.num_seqs, max_new_tokens
+        S, T, dev = batch.num_seqs, max_new_tokens, self._device_of(batch)
         self.check(lib().flat_paged_batch_reserve(
-            self.h, batch.ref, _ptr(new_lens, S, "new_lens"), _ptr(depths, T, "depths"), T, _ptr(page_counts_out, S, "page_counts_out"),
-            _ptr(free_count_out, 1, "free_count_out"), _ptr(context_lens_out, S, "context_lens_out"), _ptr(new_offsets, S + 1, "new_offsets"),
-            _ptr(slot_map, T, "slot_map"), _ptr(positions, T, "positions")))
+            self.h, batch.ref, _ptr(new_lens, S, "new_lens", dev), _ptr(depths, T, "depths", dev), T, _ptr(page_counts_out, S, "page_counts_out", dev),
+            _ptr(free_count_out, 1, "free_count_out", dev), _ptr(context_lens_out, S, "context_lens_out", dev), _ptr(new_offsets, S + 1, "new_offsets", dev),
+            _ptr(slot_map, T, "slot_map", dev), _ptr(positions, T, "positions", dev)))
 
     def paged_batch_release(self, batch: "PagedBatch", keep_lens, page_counts_out=None, free_count_out=None):
         """Gives back each sequence's pages behind its first keep_lens[s] tokens (flat_paged_batch_release)."""
-        S = batch.num_seqs
-        self.check(lib().flat_paged_batch_release(self.h, batch.ref, _ptr(keep_lens, S, "keep_lens"), _ptr(page_counts_out, S, "page_counts_out"),
-                                                  _ptr(free_count_out, 1, "free_count_out")))
+        S, dev = batch.num_seqs, self._device_of(batch)
+        self.check(lib().flat_paged_batch_release(self.h, batch.ref, _ptr(keep_lens, S, "keep_lens", dev), _ptr(page_counts_out, S, "page_counts_out", dev),
+                                                  _ptr(free_count_out, 1, "free_count_out", dev)))
 
     def paged_kv_write(self, kv_heads: int, head_dim: int, slot_map, positions, theta: float, k_source, v_source, k, v):
         """New tokens' K (turned at `positions`; None: as it is) and V into the pool rows that slot_map names (flat_paged_kv_write).
         k_source / v_source [tokens, kv_heads*head_dim], k / v [pool_rows, kv_heads*head_dim]."""
-        tokens = slot_map.numel()
-        slots, at = _ptr(slot_map, tokens, "slot_map"), _ptr(positions, tokens, "positions")
-        dtype, buffers = _buffers(k_source, v_source, k, v)
+        tokens, dev = slot_map.numel(), self.device
+        slots, at = _ptr(slot_map, tokens, "slot_map", dev), _ptr(positions, tokens, "positions", dev)
+        dtype, buffers = _buffers(dev, k_source, v_source, k, v)
         if dtype is None:
             raise FlatAttentionError(26, "one of the tensors has to tell the type")
         row = kv_heads * head_dim * (4 if dtype == F32 else 2)
@@ -514,28 +519,28 @@ class Context:
         """Attention of drafted tokens, packed sequence by sequence in `q` [tokens, q_heads*head_dim], over the cache that holds
         them behind each sequence's live tokens (flat_decode_paged_tree).  tree_mask: int32 [tokens, words] of bits, or None.  `out`:
         create_decode_output_buffer(dtype, tokens, q_heads, head_dim)."""
-        tokens = q_positions.numel()
-        offsets, at = _ptr(q_offsets, batch.num_seqs + 1, "q_offsets"), _ptr(q_positions, tokens, "q_positions")
+        tokens, dev = q_positions.numel(), self._device_of(batch)
+        offsets, at = _ptr(q_offsets, batch.num_seqs + 1, "q_offsets", dev), _ptr(q_positions, tokens, "q_positions", dev)
         words = 0
         if tree_mask is not None:
             if tree_mask.dim() != 2 or tree_mask.shape[0] != tokens:
                 raise FlatAttentionError(7, f"tree_mask has shape {tuple(tree_mask.shape)}, expected [{tokens}, words]")
             words = tree_mask.shape[1]
-        dtype, buffers = _buffers(q, k, v)
+        dtype, buffers = _buffers(dev, q, k, v)
         self.check(lib().flat_decode_paged_tree(self.h, batch.dtype if dtype is None else dtype, batch.ref, q_heads, kv_heads, head_dim, tokens, max_nodes,
-                                                max_context, offsets, at, _ptr(tree_mask, tokens * words, "tree_mask"), words, C.byref(cfg), theta, *buffers,
-                                                _whole(out)))
+                                                max_context, offsets, at, _ptr(tree_mask, tokens * words, "tree_mask", dev), words, C.byref(cfg), theta, *buffers,
+                                                _whole(dev, out)))
 
     def paged_kv_accept(self, batch: "PagedBatch", kv_heads: int, head_dim: int, accept_nodes, accept_lens, context_lens_out, k, v):
         """Moves the rows of each sequence's accepted path (accept_nodes [num_seqs, max_accept], the first accept_lens[s] of a row) behind
         its live tokens and lengthens it (flat_paged_kv_accept); context_lens_out None: in place."""
         if accept_nodes.dim() != 2 or accept_nodes.shape[0] != batch.num_seqs:
             raise FlatAttentionError(7, f"accept_nodes has shape {tuple(accept_nodes.shape)}, expected [{batch.num_seqs}, max_accept]")
-        S = batch.num_seqs
-        nodes = _ptr(accept_nodes, 0, "accept_nodes")
-        dtype, buffers = _buffers(k, v)
+        S, dev = batch.num_seqs, self._device_of(batch)
+        nodes = _ptr(accept_nodes, 0, "accept_nodes", dev)
+        dtype, buffers = _buffers(dev, k, v)
         self.check(lib().flat_paged_kv_accept(self.h, batch.dtype if dtype is None else dtype, batch.ref, kv_heads, head_dim,
-                                              accept_nodes.shape[1], nodes, _ptr(accept_lens, S, "accept_lens"), _ptr(context_lens_out, S, "context_lens_out"), *buffers))
+                                              accept_nodes.shape[1], nodes, _ptr(accept_lens, S, "accept_lens", dev), _ptr(context_lens_out, S, "context_lens_out", dev), *buffers))
 
     def chunked_prefill(self, dtype, shp, cfg, rot, query_chunk_size, q, k, v, out):
         self.check(lib().flat_chunked_prefill(self.h, C.c_int32(dtype), C.byref(shp), C.byref(cfg), C.byref(rot),
@@ -638,30 +643,38 @@ def _b(x) -> Buffer:
     return x if isinstance(x, Buffer) else buf(x)
 
 
-def _ptr(t, elements: int, name: str):
-    """Address of a contiguous int32 CUDA tensor of at least `elements`; None stays None."""
+def _ptr(t, elements: int, name: str, device: int):
+    """Address of a contiguous int32 tensor of at least `elements` on that device; None stays None."""
     if t is None:
         return None
-    if t.dtype is not _int32 or not t.is_cuda or not t.is_contiguous() or t.numel() < elements:
-        _ints(elements, **{name: t})
+    if t.dtype is not _int32 or t.get_device() != device or not t.is_contiguous() or t.numel() < elements:
+        _ints(elements, device, **{name: t})
     return t.data_ptr()
 
 
-def _ints(elements: int, **tensors):
-    """Each given tensor is a contiguous int32 CUDA tensor of at least `elements`."""
+def _ints(elements: int, device: int, **tensors):
+    """Each given tensor is a contiguous int32 tensor of at least `elements` on that device."""
     int32 = _torch().int32
     for name, t in tensors.items():
-        if t is None or (t.dtype is int32 and t.is_cuda and t.is_contiguous() and t.numel() >= elements):
+        if t is None or (t.dtype is int32 and t.get_device() == device and t.is_contiguous() and t.numel() >= elements):
             continue
         if t.dtype is not int32:
             raise FlatAttentionError(26, f"{name} must be int32, is {t.dtype}")
         if not t.is_cuda or not t.is_contiguous():
             raise FlatAttentionError(29, f"{name} must be a contiguous CUDA tensor")
+        _on(device, t, name)
         raise FlatAttentionError(22, f"{name} has {t.numel()} elements, requires {elements}")
 
 
-def _buffers(*tensors):
-    """(dtype code, flat_buffer of each): contiguous CUDA tensors of one type, or flat_buffer views, which have none (all views: None)."""
+def _on(device: int, t, name: str):
+    """Kernels take addresses of one device; another one's would be a fault."""
+    if t.get_device() != device:
+        raise FlatAttentionError(29, f"{name} is on cuda:{t.get_device()}, the call on cuda:{device}")
+
+
+def _buffers(device: int, *tensors):
+    """(dtype code, flat_buffer of each): contiguous tensors of one type on that device, or flat_buffer views, which have no type (all
+    views: None)."""
     first, buffers = None, []
     for x in tensors:
         if type(x) is not Buffer:
@@ -670,17 +683,19 @@ def _buffers(*tensors):
                 first, code = dtype, _dtype_of(x)
             elif dtype is not first:
                 raise FlatAttentionError(26, "Q, K and V differ in type")
-            x = _whole(x)
+            x = _whole(device, x)
         buffers.append(x)
     return None if first is None else code, buffers
 
 
-def _whole(x) -> Buffer:
-    """A contiguous CUDA tensor or a flat_buffer view."""
+def _whole(device: int, x) -> Buffer:
+    """A contiguous tensor on that device or a flat_buffer view."""
     if type(x) is Buffer:
         return x
-    if not x.is_cuda or not x.is_contiguous():
-        raise FlatAttentionError(29, "tensors must be contiguous and on the device")
+    if x.get_device() != device or not x.is_contiguous():
+        if not x.is_cuda or not x.is_contiguous():
+            raise FlatAttentionError(29, "tensors must be contiguous and on the device")
+        _on(device, x, "a tensor")
     return Buffer(x.data_ptr(), x.nbytes)
 
 
@@ -689,7 +704,7 @@ class PagedBatch:
     Tensors that are not given start empty: no sequence holds a page, and all pages of the pool are free, the lowest on top.
 
     The five tensors may be replaced (`batch.page_counts = counts_out` after a call out of place): later calls use the new one, a
-    captured graph keeps the old one's address.  The sizes are fixed."""
+    captured graph keeps the old one's address.  The sizes are fixed, and so is the device: that of the given tensors, or `device`."""
 
     SIZES = ("num_seqs", "page_size", "physical_pages", "max_pages_per_seq")
     TENSORS = ("page_tables", "page_counts", "context_lens", "free_pages", "free_count")
@@ -697,7 +712,9 @@ class PagedBatch:
     def __init__(self, num_seqs: int, page_size: int, physical_pages: int, max_pages_per_seq: int, page_tables=None, page_counts=None,
                  context_lens=None, free_pages=None, free_count=None, device: int = 0, dtype: int = BF16):
         torch = _torch()
-        on = dict(dtype=torch.int32, device=f"cuda:{device}")
+        given = [t for t in (page_tables, page_counts, context_lens, free_pages, free_count) if t is not None]
+        self.device = given[0].get_device() if given and given[0].is_cuda else device
+        on = dict(dtype=torch.int32, device=f"cuda:{self.device}")
         self.raw = PagedBatchRaw(num_seqs, page_size, physical_pages, max_pages_per_seq)
         self.ref = C.byref(self.raw)
         self.dtype = dtype  # of the pool, where calls are given flat_buffer views instead of tensors
@@ -713,9 +730,9 @@ class PagedBatch:
             need = {"page_tables": self.num_seqs * self.max_pages_per_seq, "free_pages": self.physical_pages, "free_count": 1}.get(name, self.num_seqs)
             if value is None:
                 raise FlatAttentionError(27, f"{name} is None")
-            _ints(need, **{name: value})
+            _ints(need, self.device, **{name: value})
             setattr(self.raw, name, value.data_ptr())
-        elif name in self.SIZES and name in self.__dict__:
+        elif (name in self.SIZES or name == "device") and name in self.__dict__:
             raise AttributeError(f"{name} of a PagedBatch is fixed")
         object.__setattr__(self, name, value)
 

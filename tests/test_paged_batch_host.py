@@ -66,3 +66,74 @@ def test_the_sizes_of_a_batch_are_fixed(name):
     with pytest.raises(AttributeError):
         setattr(b, name, 1)
     assert getattr(b, name) == getattr(b.raw, name)
+
+
+# ---- tensors of another device: the kernels would take their addresses ------------------------------
+
+class Values(Ints):
+    def __init__(self, *shape, dtype=torch.bfloat16, device=0):
+        super().__init__(*shape, dtype=dtype, device=device)
+
+    @property
+    def nbytes(self):
+        return self.numel() * torch.empty(0, dtype=self.dtype).element_size()
+
+
+def context(device=0):
+    """A context that has only got as far as its device: what is refused is refused before the library is called."""
+    c = fa.Context.__new__(fa.Context)
+    c.device, c.h = device, None
+    return c
+
+
+def calls(c, b, odd, d=0):
+    """(tensors, call) of each entry point; the tensor number `odd` is on another device."""
+    def on(tensors):
+        made = [t(device=d + (i == odd)) for i, t in enumerate(tensors)]
+        return made
+    i = lambda *n: (lambda device: Ints(*n, device=device))  # noqa: E731
+    v = lambda *n: (lambda device: Values(*n, device=device))  # noqa: E731
+    out = lambda device: Values(4096, dtype=torch.uint8, device=device)  # noqa: E731
+    cfg = fa.config(True)
+    return {
+        "reserve": ([i(2), i(3), i(6), i(6), i(6), i(2), i(1), i(2)],
+                    lambda x: c.paged_batch_reserve(b, x[0], 6, x[1], x[2], x[3], x[4], x[5], x[6], x[7])),
+        "release": ([i(2), i(2), i(1)], lambda x: c.paged_batch_release(b, *x)),
+        "write": ([i(3), i(3), v(3, 128), v(3, 128), v(32, 128), v(32, 128)], lambda x: c.paged_kv_write(2, 64, x[0], x[1], 1e4, *x[2:])),
+        "tree": ([i(3), i(3), i(3, 1), v(3, 256), v(32, 128), v(32, 128), out],
+                 lambda x: c.decode_paged_tree(b, 4, 2, 64, 3, 9, x[0], x[1], x[2], cfg, 1e4, *x[3:])),
+        "accept": ([i(2, 3), i(2), i(2), v(32, 128), v(32, 128)], lambda x: c.paged_kv_accept(b, 2, 64, *x)),
+    }, on
+
+
+@pytest.mark.parametrize("name", ["reserve", "release", "write", "tree", "accept"])
+@pytest.mark.parametrize("device", [0, 1])
+def test_tensors_of_another_device_than_the_context_s_are_refused(name, device):
+    c, b = context(device), batch(device=device)
+    for odd in range(len(calls(c, b, None)[0][name][0])):
+        table, on = calls(c, b, odd, device)
+        tensors, call = table[name]
+        with pytest.raises(fa.FlatAttentionError) as e:
+            call(on(tensors))
+        assert e.value.kind == "UnsupportedShape" and f"is on cuda:{device + 1}" in e.value.detail, odd
+
+
+@pytest.mark.parametrize("name", ["reserve", "release", "tree", "accept"])
+def test_a_batch_of_another_device_than_the_context_s_is_refused(name):
+    c, b = context(0), batch(device=1)
+    table, on = calls(c, b, None)
+    with pytest.raises(fa.FlatAttentionError) as e:
+        table[name][1](on(table[name][0]))
+    assert e.value.kind == "UnsupportedShape" and "the batch is on cuda:1" in e.value.detail
+
+
+def test_the_tensors_of_a_batch_are_on_one_device():
+    assert batch(device=3).device == 3
+    with pytest.raises(fa.FlatAttentionError) as e:
+        batch(free_count=Ints(1, device=1))
+    assert e.value.kind == "UnsupportedShape" and "free_count is on cuda:1" in e.value.detail
+    b = batch()
+    with pytest.raises(fa.FlatAttentionError):
+        b.context_lens = Ints(2, device=1)
+    with pytest.raises(AttributeError):
+        b.device = 1
