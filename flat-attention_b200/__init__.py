@@ -731,6 +731,8 @@ class PagedBatch:
             if value is None:
                 raise FlatAttentionError(27, f"{name} is None")
             _ints(need, self.device, **{name: value})
+            if name == "page_tables" and value.dim() > 1 and value.shape[-1] != self.max_pages_per_seq:
+                raise FlatAttentionError(7, f"rows of page_tables have {value.shape[-1]} entries, expected {self.max_pages_per_seq}")
             setattr(self.raw, name, value.data_ptr())
         elif (name in self.SIZES or name == "device") and name in self.__dict__:
             raise AttributeError(f"{name} of a PagedBatch is fixed")

@@ -137,3 +137,15 @@ def test_the_tensors_of_a_batch_are_on_one_device():
         b.context_lens = Ints(2, device=1)
     with pytest.raises(AttributeError):
         b.device = 1
+
+
+# ---- shapes that the number of elements alone does not tell ------------------------------------------
+
+def test_a_page_table_with_rows_of_another_length_is_refused():
+    """Row s would be read from the middle of another one."""
+    assert batch(page_tables=Ints(6)).raw.page_tables == 0x1000  # flat: as many as there have to be
+    assert batch(page_tables=Ints(5, 3)).raw.page_tables == 0x1000  # rows that the batch does not use
+    for shape in ((2, 4), (3, 2), (2, 1, 6)):
+        with pytest.raises(fa.FlatAttentionError) as e:
+            batch(page_tables=Ints(*shape))
+        assert e.value.kind == "LengthMismatch"
