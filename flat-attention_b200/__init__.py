@@ -526,6 +526,8 @@ class Context:
             if tree_mask.dim() != 2 or tree_mask.shape[0] != tokens:
                 raise FlatAttentionError(7, f"tree_mask has shape {tuple(tree_mask.shape)}, expected [{tokens}, words]")
             words = tree_mask.shape[1]
+            if words == 0:  # it has no address, which would be no mask
+                raise FlatAttentionError(7, f"tree_mask rows of 0 words do not hold {max_nodes} drafted tokens")
         dtype, buffers = _buffers(dev, q, k, v)
         self.check(lib().flat_decode_paged_tree(self.h, batch.dtype if dtype is None else dtype, batch.ref, q_heads, kv_heads, head_dim, tokens, max_nodes,
                                                 max_context, offsets, at, _ptr(tree_mask, tokens * words, "tree_mask", dev), words, C.byref(cfg), theta, *buffers,

@@ -149,3 +149,12 @@ def test_a_page_table_with_rows_of_another_length_is_refused():
         with pytest.raises(fa.FlatAttentionError) as e:
             batch(page_tables=Ints(*shape))
         assert e.value.kind == "LengthMismatch"
+
+
+def test_a_mask_without_words_is_refused():
+    """An empty tensor has the address 0, which is the call without a mask."""
+    c, b = context(), batch()
+    with pytest.raises(fa.FlatAttentionError) as e:
+        c.decode_paged_tree(b, 4, 2, 64, 3, 9, Ints(3), Ints(3), Ints(3, 0, at=0), fa.config(True), 1e4, Values(3, 256), Values(32, 128), Values(32, 128),
+                            Values(4096, dtype=torch.uint8))
+    assert e.value.kind == "LengthMismatch"
