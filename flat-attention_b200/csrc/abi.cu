@@ -783,17 +783,27 @@ int32_t flat_ctx_device_status(flat_ctx *ctx) {
     DeviceStatus h{};
     FLAT_CUDA_OK(ctx, cudaStreamSynchronize(ctx->stream));
     FLAT_CUDA_OK(ctx, cudaMemcpy(&h, ctx->dev_status, sizeof h, cudaMemcpyDeviceToHost));
-    const int code = (int)(h.word >> 32), where = (int)(uint32_t)h.word;
+    const int code = (int)(h.word >> 48), place = (int)(h.word >> 32 & 0xffff), where = (int)(uint32_t)h.word;
     if (code != 0) {
         const DeviceGuard guard(ctx);
-        if (code == FLAT_ERR_PAGE_OUT_OF_RANGE)
+        if (code == FLAT_ERR_PAGE_OUT_OF_RANGE && place == kPlacePages)
+            fail(ctx, code, "a page of sequence %d lies outside the physical pool", where);
+        else if (code == FLAT_ERR_PAGE_OUT_OF_RANGE && place == kPlaceSlot)
+            fail(ctx, code, "the slot of token %d lies behind the pool; the token was left out", where);
+        else if (code == FLAT_ERR_PAGE_OUT_OF_RANGE && place == kPlaceBound)
+            fail(ctx, code, "sequence %d has more tokens than its pages or max_context hold; those behind were left out", where);
+        else if (code == FLAT_ERR_PAGE_OUT_OF_RANGE)
             fail(ctx, code, "a page-table entry of sequence %d lies outside the physical pool; its tokens were masked", where);
         else if (code == FLAT_ERR_NON_FINITE_INPUT)
             fail(ctx, code, "a device-side input scan found a non-finite value (tensor %d)", where);
         else if (code == FLAT_ERR_CAPACITY_EXCEEDED)
             fail(ctx, code, "the free pages do not hold the new tokens of sequence %d", where);
+        else if (code == FLAT_ERR_CAPACITY_OVERFLOW && where < 0)
+            fail(ctx, code, "the count of free pages lies outside the pool");
         else if (code == FLAT_ERR_CAPACITY_OVERFLOW)
-            fail(ctx, code, "the count of free pages leaves the pool (sequence %d)", where);
+            fail(ctx, code, "the pool has no room for the pages that sequence %d gives back; they were dropped", where);
+        else if (code == FLAT_ERR_LENGTH_MISMATCH && place == kPlacePath)
+            fail(ctx, code, "the accepted path of sequence %d does not rise, is too long or leaves its pages; nothing of it was moved", where);
         else if (code == FLAT_ERR_INVALID_CACHE_LENGTH || code == FLAT_ERR_LENGTH_MISMATCH)
             fail(ctx, code, "lengths of sequence %d do not fit its pages or the call's bounds; it was left out", where);
         else

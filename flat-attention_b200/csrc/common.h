@@ -21,10 +21,17 @@ constexpr int kMaxHeadDim = 128;  // WGSL_MAX_HEAD_DIM, src/lib.rs:60
 constexpr uint64_t kShortPartialBytes = 32ull << 20;  // 508 parts of 32 heads at D = 128
 constexpr uint64_t kF32TableBytes = 16ull << 20;  // 32768 positions at head_dim 128
 
-// Status word of a context, written by kernels and 0 where there is nothing to report: a FLAT_ERR_* code in the upper half, in the lower one
-// which wait gave up (a tag of the kernel) or which sequence or entry of the call is meant.
+// Status word of a context, written by kernels and 0 where there is nothing to report: a FLAT_ERR_* code in the upper 16 bits, a StatusPlace in
+// the next 16, in the lower half which wait gave up (a tag of the kernel) or which sequence or token of the call is meant.
 struct DeviceStatus {
     unsigned long long word;
+};
+enum StatusPlace {
+    kPlaceSequence = 0,  // an entry of a sequence's page table that attention met, or its lengths
+    kPlacePages = 1,     // a page that reserve or release met
+    kPlaceSlot = 2,      // the slot of a token
+    kPlaceBound = 3,     // tokens of a sequence behind max_context or without a page
+    kPlacePath = 4,      // the accepted path of a sequence
 };
 
 }  // namespace flat
@@ -169,8 +176,8 @@ __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepco
 __device__ __forceinline__ void grid_dependency_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // The largest word stays, whichever comes last: a code and its place belong together, what is named does not depend on the order of the
 // blocks, and a wait that gave up, whose code is the largest that a kernel reports, is not hidden by a bad page.
-__device__ __forceinline__ void report_status(DeviceStatus *status, int code, int where) {
-    atomicMax(&status->word, (unsigned long long)(unsigned)code << 32 | (unsigned)where);
+__device__ __forceinline__ void report_status(DeviceStatus *status, int code, int where, StatusPlace place = kPlaceSequence) {
+    atomicMax(&status->word, (unsigned long long)(unsigned)code << 48 | (unsigned long long)place << 32 | (unsigned)where);
 }
 #endif
 

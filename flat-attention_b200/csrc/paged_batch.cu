@@ -155,7 +155,7 @@ __device__ __forceinline__ NewToken reserve_look(const PagedBatchParams &p, cons
 }
 __device__ __forceinline__ int reserve_enter(const PagedBatchParams &p, NewToken x) {  // the token's slot
     if (x.seq >= 0 && (unsigned)x.page >= (unsigned)p.physical_pages) {
-        report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, x.seq);
+        report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, x.seq, kPlacePages);
         x.page = -1;
     }
     if (x.entry >= 0) p.page_tables[x.entry] = x.page;
@@ -196,7 +196,7 @@ __device__ __forceinline__ void release_scan(const PagedBatchParams &p) {
 __device__ __forceinline__ void release_page(const PagedBatchParams &p, int i, int f) {
     const int s = sequence_of(p.plan_offsets, p.num_seqs, i);
     const int page = p.page_tables[(int64_t)s * p.max_pages + p.plan[s].y - 1 - (i - p.plan_offsets[s])];
-    if ((unsigned)page >= (unsigned)p.physical_pages) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, s);
+    if ((unsigned)page >= (unsigned)p.physical_pages) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, s, kPlacePages);
     p.free_pages[f + i] = page;
 }
 
@@ -334,7 +334,7 @@ template <bool RELEASE> __global__ void __launch_bounds__(kScanThreads) paged_ba
 #pragma unroll
             for (int u = 0; u < kItems; ++u) {
                 if (u >= n) break;
-                if ((unsigned)page[u] >= (unsigned)p.physical_pages) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, seq[u]);
+                if ((unsigned)page[u] >= (unsigned)p.physical_pages) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, seq[u], kPlacePages);
                 p.free_pages[f + i0 + u] = page[u];
             }
         } else {

@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(kThreads) paged_write_kernel(const __grid_cons
     const int n = (int)min((int64_t)p.block_tokens, p.tokens - first);
     if (threadIdx.x < n) {
         const int slot = p.slots[first + threadIdx.x];
-        if (slot >= p.pool_rows) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, (int)(first + threadIdx.x));
+        if (slot >= p.pool_rows) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, (int)(first + threadIdx.x), kPlaceSlot);
         row_s[threadIdx.x] = slot < p.pool_rows ? slot : -1;
     }
     const int total = n * vecs;
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kThreads) paged_write_pairs_kernel(const __gri
         const int64_t row = p.slots[t];
         if (row < 0) continue;
         if (row >= p.pool_rows) {
-            if (e == 0) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, (int)t);
+            if (e == 0) report_status(p.status, FLAT_ERR_PAGE_OUT_OF_RANGE, (int)t, kPlaceSlot);
             continue;
         }
         const bool two = e + 1 < p.row_elems;
@@ -174,7 +174,7 @@ template <typename V> __global__ void __launch_bounds__(kThreads) paged_accept_k
     const bool bad = bad_s != 0;
     if (threadIdx.x == 0) p.context_lens_out[seq] = bad ? len : len + take;  // may be context_lens: every thread has read the length
     if (bad) {
-        if (threadIdx.x == 0) report_status(p.status, FLAT_ERR_LENGTH_MISMATCH, seq);
+        if (threadIdx.x == 0) report_status(p.status, FLAT_ERR_LENGTH_MISMATCH, seq, kPlacePath);
         return;
     }
     for (int base = 0; base < take; base += kSteps) {

@@ -43,7 +43,7 @@ template <> __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bf
 
 __device__ __forceinline__ TreeSequence span_of(const TreeParams &p, int seq) {
     const TreeSequence s = tree_sequence(p, seq);
-    if (s.code && threadIdx.x == 0) report_status(p.status, s.code, seq);
+    if (s.code && threadIdx.x == 0) report_status(p.status, s.code, seq, kPlaceBound);
     return s;
 }
 

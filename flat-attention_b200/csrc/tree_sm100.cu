@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const 
             if (base + (int)threadIdx.x < p.t.num_seqs) {
                 mine = tree_sequence(p.t, base + threadIdx.x);
                 units = units_of<ROWS>(p, mine, grain);
-                if (mine.code && counting && blockIdx.x == 0) report_status(p.t.status, mine.code, base + threadIdx.x);
+                if (mine.code && counting && blockIdx.x == 0) report_status(p.t.status, mine.code, base + threadIdx.x, kPlaceBound);
             }
             int upto = units;
 #pragma unroll

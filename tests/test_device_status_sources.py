@@ -24,7 +24,7 @@ def test_kernels_write_the_status_word_through_one_function_only():
     body = text("common.h")
     body = body[body.index("void report_status("):]
     body = body[:body.index("}\n")]
-    assert body.count(";") == 1 and "atomicMax(&status->word," in body and re.search(r"code << 32 \|[^;]*where\)", body)
+    assert body.count(";") == 1 and "atomicMax(&status->word," in body and re.search(r"code << 48 \|[^;]*where\)", body)
 
 
 def test_a_wait_that_gave_up_has_the_largest_code_that_kernels_report():

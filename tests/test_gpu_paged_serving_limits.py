@@ -104,6 +104,57 @@ def test_what_the_status_names_does_not_depend_on_the_order_of_the_blocks():
         assert "1999" in fa.lib().flat_last_error_detail(c.h).decode()
 
 
+def told(c, kind):
+    """What the status says, once: its words."""
+    assert fa.STATUS[c.device_status()] == kind
+    text = fa.lib().flat_last_error_detail(c.h).decode()
+    assert c.device_status() == 0
+    return text
+
+
+@pytest.mark.parametrize("shape", [(fa.F32, 4, 2, 64, 16), (fa.BF16, 8, 2, 128, 16)], ids=str)
+def test_the_words_of_a_fault_of_the_attention_name_what_was_met(shape):
+    c = ctx()
+    t = TreeCase(12, *shape, [60, 90], [6, 4])
+    t.run(c, max_context=80, status=35)
+    assert "sequence 1 has more tokens than its pages or max_context hold" in fa.lib().flat_last_error_detail(c.h).decode()
+    t.held[0] -= 1
+    t.run(c, status=35)
+    assert "sequence 0 has more tokens" in fa.lib().flat_last_error_detail(c.h).decode()
+    t.held[0] += 1
+    bad = t.table.copy()
+    bad[1, 2] = t.pool
+    t.run(c, table=bad, status=35)
+    assert "a page-table entry of sequence 1 lies outside the physical pool" in fa.lib().flat_last_error_detail(c.h).decode()
+    t.run(c, max_nodes=5, status=7)
+    assert "lengths of sequence 0 do not fit" in fa.lib().flat_last_error_detail(c.h).decode()
+
+
+def test_the_words_of_a_fault_of_the_other_calls_name_what_was_met():
+    c = ctx()
+    write_behind_the_pool(c, [7])
+    assert "the slot of token 7 lies behind the pool" in told(c, "PageOutOfRange")
+    src, pool = torch.ones(3, 6, device="cuda"), torch.zeros(8, 6, device="cuda")  # rows that are not whole vectors
+    c.paged_kv_write(1, 6, i32([1, 9, 2]), None, THETA, src, src, pool, pool.clone())
+    assert "the slot of token 1 lies behind the pool" in told(c, "PageOutOfRange")
+    k = torch.zeros(32, 8, device="cuda")
+    b = fa.PagedBatch(2, 4, 8, 3, i32([[3, 1, 0], [2, 4, 9]]), i32([2, 2]), i32([2, 1]))
+    c.paged_kv_accept(b, 1, 8, i32([[0, 1], [1, 1]]), i32([2, 2]), None, k, k.clone())
+    assert "the accepted path of sequence 1 does not rise" in told(c, "LengthMismatch")
+    b = fa.PagedBatch(2, 4, 8, 3, i32([[3, 1, 0], [2, 99, 9]]), i32([1, 2]), i32([2, 1]), i32([0, 4, 5, 6, 7, 0, 0, 0]), i32([5]))
+    c.paged_batch_release(b, i32([4, 0]))
+    assert "a page of sequence 1 lies outside the physical pool" in told(c, "PageOutOfRange")
+    b = fa.PagedBatch(2, 4, 8, 3, i32([[3, 1, 0], [2, 4, 9]]), i32([2, 2]), i32([2, 1]), i32([0] * 8), i32([8]))
+    c.paged_batch_release(b, i32([8, 0]))
+    assert "no room for the pages that sequence 1 gives back" in told(c, "CapacityOverflow")
+    b.free_count = i32([9])
+    c.paged_batch_release(b, i32([8, 0]))
+    assert "the count of free pages lies outside the pool" in told(c, "CapacityOverflow")
+    b = fa.PagedBatch(2, 4, 8, 3, i32([[3, 1, 0], [2, 4, 9]]), i32([2, 2]), i32([2, 1]), i32([0] * 8), i32([0]))
+    c.paged_batch_reserve(b, i32([0, 9]), 9, i32([0] * 3), i32([0] * 9), i32([0] * 9))
+    assert "the free pages do not hold the new tokens of sequence 1" in told(c, "CapacityExceeded")
+
+
 # ---- results of a call out of place that take the place of the batch's tensors -----------------------
 
 def test_counts_written_out_of_place_are_used_once_they_are_the_batch_s():
