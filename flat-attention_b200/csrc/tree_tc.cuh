@@ -81,11 +81,6 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap *map
         : "memory");
 }
 
-__device__ __forceinline__ void tma_prefetch_5d(const CUtensorMap *map, int group, int head) {
-    asm volatile("cp.async.bulk.prefetch.tensor.5d.L2.global.tile [%0, {%1, %1, %1, %2, %3}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(group), "r"(head)
-                 : "memory");
-}
-
 // Order of the tiles of a segment of n tiles in the ring: the first `ahead` K tiles, then V tile v and K tile v + ahead for each v.
 __device__ __forceinline__ int k_entry(int i, int ahead) { return i < ahead ? i : 2 * i - ahead + 1; }
 __device__ __forceinline__ int v_entry(int v, int n, int ahead) { return min(n, ahead) + v + min(v, max(0, n - ahead)); }
@@ -187,10 +182,6 @@ __device__ __forceinline__ void add_not_finite(const TreeParams &p, const TreeSe
             if (!isfinite(y)) o[e] += y;
         }
     }
-}
-
-__device__ __forceinline__ int64_t quotient(int64_t x, int64_t d) {  // x >= 0, d > 0; in 32 bits where they hold both
-    return (x | d) >> 32 ? x / d : (int64_t)((uint32_t)x / (uint32_t)d);
 }
 
 // 5-D map over (64 dims, token of 8, 64-dim block, group of 8 tokens, head) of a pool, with a box of one head's `box_rows` tokens.
