@@ -174,6 +174,12 @@ inline bool may_overlap_previous(flat_ctx *ctx) {
 #ifdef __CUDACC__
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename T> __device__ __forceinline__ float to_float(T x);
+template <> __device__ __forceinline__ float to_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 // The largest word stays, whichever comes last: a code and its place belong together, what is named does not depend on the order of the
 // blocks, and a wait that gave up, whose code is the largest that a kernel reports, is not hidden by a bad page.
 __device__ __forceinline__ void report_status(DeviceStatus *status, int code, int where, StatusPlace place = kPlaceSequence) {

@@ -96,13 +96,6 @@ __global__ void __launch_bounds__(kThreads) paged_write_kernel(const __grid_cons
     }
 }
 
-template <typename T> __device__ __forceinline__ float to_float(T x);
-template <> __device__ __forceinline__ float to_float<float>(float x) { return x; }
-template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_float(float x);
-template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
 // Any head_dim and alignment: a thread takes one pair of a row.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) paged_write_pairs_kernel(const __grid_constant__ PagedWriteParams p) {

@@ -19,13 +19,6 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kRows = 32, kTokens = 32, kThreads = 128, kMaxSplits = 256;
 constexpr float kMasked = -1.f;  // in place of a weight, which is never negative
 
-template <typename T> __device__ __forceinline__ float to_float(T x);
-template <> __device__ __forceinline__ float to_float<float>(float x) { return x; }
-template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_float(float x);
-template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
 // Four values from `at` on as f32, `left` of them there; vec: rows are whole aligned groups of four.
 template <typename T> __device__ __forceinline__ float4 load4(const T *at, bool vec, int left);
 template <> __device__ __forceinline__ float4 load4<float>(const float *at, bool vec, int left) {

@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_sm100_kernel(const 
         }
     }
     __syncthreads();
-    grid_dependency_wait();  // long over
+    grid_dependency_wait();  // long over: it stands here so that the rule, nothing is let in before one's own wait, can be seen
     grid_dependency_launch();
     const uint32_t tmem_base = ctl.tmem;
     auto col_s = [](int b) { return (uint32_t)(D + b * kTok); };  // O in columns 0 .. D - 1
