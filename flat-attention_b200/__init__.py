@@ -481,16 +481,16 @@ class Context:
                                             C.c_uint64(head_dim), buf(partial_o), buf(partial_lse), buf(out)))
 
     # ---- batches whose lengths and page tables stay on the device ----
-    def _device_of(self, batch: "PagedBatch") -> int:
-        if batch.device != self.device:
-            raise FlatAttentionError(29, f"the batch is on cuda:{batch.device}, the context on cuda:{self.device}")
-        return self.device
+    def _other_device(self, batch: "PagedBatch"):
+        raise FlatAttentionError(29, f"the batch is on cuda:{batch.device}, the context on cuda:{self.device}")
 
     def paged_batch_reserve(self, batch: "PagedBatch", new_lens, max_new_tokens: int, new_offsets, slot_map, positions, depths=None,
                             page_counts_out=None, free_count_out=None, context_lens_out=None):
         """Pages and slots for new_lens[s] tokens behind each sequence's live ones (flat_paged_batch_reserve); outputs None: in place,
         context_lens_out None: not written."""
-        S, T, dev = batch.num_seqs, max_new_tokens, self._device_of(batch)
+        S, T, dev = batch.num_seqs, max_new_tokens, self.device
+        if batch.device != dev:
+            self._other_device(batch)
         self.check(lib().flat_paged_batch_reserve(
             self.h, batch.ref, _ptr(new_lens, S, "new_lens", dev), _ptr(depths, T, "depths", dev), T, _ptr(page_counts_out, S, "page_counts_out", dev),
             _ptr(free_count_out, 1, "free_count_out", dev), _ptr(context_lens_out, S, "context_lens_out", dev), _ptr(new_offsets, S + 1, "new_offsets", dev),
@@ -498,7 +498,9 @@ class Context:
 
     def paged_batch_release(self, batch: "PagedBatch", keep_lens, page_counts_out=None, free_count_out=None):
         """Gives back each sequence's pages behind its first keep_lens[s] tokens (flat_paged_batch_release)."""
-        S, dev = batch.num_seqs, self._device_of(batch)
+        S, dev = batch.num_seqs, self.device
+        if batch.device != dev:
+            self._other_device(batch)
         self.check(lib().flat_paged_batch_release(self.h, batch.ref, _ptr(keep_lens, S, "keep_lens", dev), _ptr(page_counts_out, S, "page_counts_out", dev),
                                                   _ptr(free_count_out, 1, "free_count_out", dev)))
 
@@ -519,7 +521,9 @@ class Context:
         """Attention of drafted tokens, packed sequence by sequence in `q` [tokens, q_heads*head_dim], over the cache that holds
         them behind each sequence's live tokens (flat_decode_paged_tree).  tree_mask: int32 [tokens, words] of bits, or None.  `out`:
         create_decode_output_buffer(dtype, tokens, q_heads, head_dim)."""
-        tokens, dev = q_positions.numel(), self._device_of(batch)
+        tokens, dev = q_positions.numel(), self.device
+        if batch.device != dev:
+            self._other_device(batch)
         offsets, at = _ptr(q_offsets, batch.num_seqs + 1, "q_offsets", dev), _ptr(q_positions, tokens, "q_positions", dev)
         words = 0
         if tree_mask is not None:
@@ -538,7 +542,9 @@ class Context:
         its live tokens and lengthens it (flat_paged_kv_accept); context_lens_out None: in place."""
         if accept_nodes.dim() != 2 or accept_nodes.shape[0] != batch.num_seqs:
             raise FlatAttentionError(7, f"accept_nodes has shape {tuple(accept_nodes.shape)}, expected [{batch.num_seqs}, max_accept]")
-        S, dev = batch.num_seqs, self._device_of(batch)
+        S, dev = batch.num_seqs, self.device
+        if batch.device != dev:
+            self._other_device(batch)
         nodes = _ptr(accept_nodes, 0, "accept_nodes", dev)
         dtype, buffers = _buffers(dev, k, v)
         self.check(lib().flat_paged_kv_accept(self.h, batch.dtype if dtype is None else dtype, batch.ref, kv_heads, head_dim,
