@@ -310,7 +310,9 @@ template <typename T> int launch(flat_ctx *ctx, TreeParams &p) {
     const int tiles = (int)(((int64_t)p.max_nodes * p.group + kRows - 1) / kRows);
     if ((int64_t)tiles * p.kv_heads > 65535)
         return fail(ctx, FLAT_ERR_DISPATCH_LIMIT, "%d drafted tokens of %d heads are more row tiles than one launch has", p.max_nodes, p.q_heads);
-    // chunks of the longest context that fill the device about four times, a tile of 32 tokens at least, as many as the scratch holds
+    // chunks of the longest context that fill the device about four times, a tile of 32 tokens at least, as many as the scratch holds; the
+    // longest that the bound allows: where the sequences are far shorter they are few chunks of many tiles (18 us -> 117 us for
+    // sequences of up to 1200 tokens under a bound of 32768)
     const int64_t rows = (int64_t)p.max_q * p.q_heads, units = (int64_t)tiles * p.kv_heads * p.num_seqs;
     const int64_t fit = (int64_t)((kPagedScratchBytes - kPagedPlanBytes) / (rows * (p.head_dim + 1) * sizeof(float)));
     int64_t splits = std::min<int64_t>({(p.max_context + kTokens - 1) / kTokens, std::max<int64_t>(1, (int64_t)ctx->sm_count * 4 / units), kMaxSplits, fit});

@@ -13,17 +13,22 @@
 //   four warps work a softmax row per thread, without shuffles, and write results, while the next item's first scores are formed;
 //   one thread issues all products.  Two score tiles alternate; P lies over the scores it comes from, and the products of one
 //   thread execute in order, so the scores after next cannot overtake the product that reads that P.
-// ROWS is 64 where no sequence has more, otherwise 128.  A product of 64 rows takes as long as one of 128, but half the power, and the
-// power limit is what a long run meets: one drafted token against 32 x 4000 takes 94 us a call in a run of seconds, with products
-// of 128 rows 119 (alone 91 and 98).  For the same reason rows that are not there are zeros.  Of more than 128 rows, two blocks of 128
-// go to two CTAs that walk the same span, so that the second one finds K and V in the L2.
+// ROWS is 64 where max_nodes allows a sequence no more, otherwise 128, whatever the sequences have (the host does not know).  A product of
+// 64 rows takes as long as one of 128, but half the power, and the power limit is what a long run meets: at head_dim 128 one drafted
+// token against 32 x 4000 takes 92 us a call in a run of seconds, with products of 128 rows 104 (alone 90 and 94), 4 to 16 tokens
+// against 32 x 512 to 8192 108 and 118 (101 and 104).  At head_dim 64, where the softmax counts for more and a warp of it has 16 rows
+// instead of 32, one token takes 62 and 65 (alone 62 both), 4 to 16 tokens 82 and 79 (82 and 75), and 16 tokens against 32 x 4000, 64
+// whole rows, 78 and 71 (74 and 62).  For the power too rows that are not there are zeros.  Of more than 128 rows, two blocks of 128 go
+// to two CTAs that walk the same span, so that the second one finds K and V in the L2.
 //
 // Work: the tiles of all items, a block of ROWS rows of a (sequence, KV head) each, stand in one line, which is cut into equal spans,
 // one per CTA, whatever the lengths are.  Every CTA adds the lengths up itself, so nothing is planned on the host.  An item that a span's end cuts is
 // joined, from the parts in order, by the CTA that finds that they are all there; everything else is written directly.
 //
-// Roundings: q enters as the sum of two bf16 numbers (the tensor core takes one type, and K is bf16; q alone would cost 2^-9 of the
-// scores: 1.7 times the error of the bf16 result, where this way is 1.4 times it), P as bf16, sums and statistics are f32.
+// Roundings: q enters as the sum of two bf16 numbers (the tensor core takes one type, and K is bf16; q alone would cost 2^-8 of the
+// scores: 1.7 times the error of the bf16 result, where this way is 1.4 times it), P as bf16 (a second summand of it would double the
+// value products; against 64 bits O is off by 2.3e-3 in the 2-norm, with weights of 32 bits by 1.7e-3, which is the result's own
+// rounding), sums and statistics are f32.
 // The running maximum is followed only when it grows by more than 2^8, which keeps the accumulator out of the loop; P then
 // reaches 2^8, sums stay far inside f32.
 //

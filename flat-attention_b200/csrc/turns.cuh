@@ -1,7 +1,7 @@
 // RoPE angles of far positions.  A frequency is held as the fraction of a turn that a position is worth, scaled by 2^64: the
 // product with a position modulo 2^64 is then the exact fraction of a turn of that product, whatever the position (negative ones
-// too), and its upper 32 bits give the angle to 2^-32 of a turn.  An angle that is formed as a 32-bit float is off by position *
-// 2^-25 radians in the fastest pair, 4e-3 at position 131072.
+// too), and its upper 32 bits, as a float, give the angle to 2^-26 of a turn (24 of 31 bits, worst near half a turn).  An angle that
+// is formed as a 32-bit float of position times frequency is off by position * 2^-25 radians in the fastest pair, 4e-3 at position 131072.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -34,7 +34,8 @@ __device__ __forceinline__ float2 turn_of(int32_t position, uint64_t turns) {
     sincospif((float)(int32_t)(phase >> 32) * 0x1p-31f, &cs.y, &cs.x);
     return cs;
 }
-// The same by the special-function unit: 2^-21 off at most, for queries that are rounded to 16 bits in two summands anyway
+// The same by the special-function unit, for queries that are rounded to 16 bits in two summands anyway.  Off by 2^-20 at most: 2^-21.2 for
+// the function itself between -pi and pi, 2^-21.4 for the angle (2^-26 of a turn, the constant and the product in 32 bits)
 __device__ __forceinline__ float2 turn_of_fast(int32_t position, uint64_t turns) {
     const uint64_t phase = turns * (uint64_t)(int64_t)position + 0x80000000ull;
     const float angle = (float)(int32_t)(phase >> 32) * (0x1p-31f * 3.14159265358979f);
