@@ -746,6 +746,10 @@ class PagedBatch:
             raise AttributeError(f"{name} of a PagedBatch is fixed")
         object.__setattr__(self, name, value)
 
+    def __copy__(self):
+        """A batch over the same tensors with addresses of its own."""
+        return PagedBatch(*(getattr(self, name) for name in self.SIZES), *(getattr(self, name) for name in self.TENSORS), dtype=self.dtype)
+
 
 # ---- PagedKvTable (src/paged_kv.rs:75-188) -----------------------------------------------------
 class PagedKvTable:

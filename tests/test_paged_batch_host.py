@@ -1,4 +1,6 @@
 """What PagedBatch and the calls that take it check on the host, with stand-ins for device tensors: nothing here needs a GPU."""
+import copy
+
 import pytest
 import torch
 
@@ -66,6 +68,16 @@ def test_the_sizes_of_a_batch_are_fixed(name):
     with pytest.raises(AttributeError):
         setattr(b, name, 1)
     assert getattr(b, name) == getattr(b.raw, name)
+
+
+def test_a_copy_of_a_batch_has_addresses_of_its_own():
+    b = batch()
+    b.dtype = fa.F32
+    other = copy.copy(b)
+    assert all(getattr(other, n) is getattr(b, n) for n in fa.PagedBatch.TENSORS) and other.dtype == fa.F32
+    old = b.raw.page_counts
+    other.page_counts = Ints(2, at=0x7770)
+    assert b.raw.page_counts == old and other.raw.page_counts == 0x7770 and b.page_counts.data_ptr() == old
 
 
 # ---- tensors of another device: the kernels would take their addresses ------------------------------
